@@ -60,7 +60,11 @@ typedef enum wuda_device_status {
     WUDA_DEV_TIMEOUT_MLA_SCORES_READ = 153,
     WUDA_DEV_TIMEOUT_MLA_PROBS = 154,
     WUDA_DEV_TIMEOUT_MLA_OUTPUT = 155,
-    WUDA_DEV_MLA_SCALE_RANGE = 156  /* a key's scale exponent outside [-15, 7] was clamped into that range */
+    WUDA_DEV_MLA_SCALE_RANGE = 156, /* a key's scale exponent outside [-15, 7] was clamped into that range */
+    WUDA_DEV_BAD_SLOT = 161,        /* a request slot outside [-1, capacity), or in a batch for the second time: its row was left out */
+    WUDA_DEV_NO_FREE_PAGE = 162,    /* a request found no free page: its row was left out */
+    WUDA_DEV_BAD_LENGTH = 163,      /* a request's length does not fit its tables, the step's buffers or its group: its row was left out */
+    WUDA_DEV_BAD_PARENT = 164       /* a beam's parent is no live beam of its group: the beam was given none */
 } wuda_device_status;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -1029,6 +1033,139 @@ int wuda_indexer_topk_host_pages(wuda_indexer_plan* plan, const void* q_host, co
                                  const int32_t* dirty_pages_host, int n_dirty, const float* weights_host,
                                  const int32_t* context_lens_host, const int32_t* block_table_host,
                                  int32_t* page_indices_host, float* logits_host, int batch, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Step tables: what a step's kernels read about its requests, computed on the device from their lengths.
+ *
+ * The host-side counterpart is the reference's KVCacheManager.step_begin / block_table / swa_indices
+ * (test/kv_cache_manager.py:53-257), whose positions, destinations and page order this gives for one token per request.
+ *
+ * Row b of a step is request slot slots[b] (-1: a padded row) with new_tokens[b] tokens (new_tokens == NULL: one each).
+ * With old = lengths[slot], now = old + new_tokens[b], entries(x) = x / ratio and pages(x) = ceil(entries(x) / entries_per_block):
+ *   free pages   the row takes pages(now) - pages(old) pages of each compressed pool from the top of its free stack
+ *                (free[count - 1] first), rows in their order, and appends them to the slot's row of the page table
+ *   token i      of the row stands at position pos = old + i.  idx_dst / cmp_dst: entry (pos + 1) / ratio - 1 through the page table
+ *                where (pos + 1) % ratio == 0; swa_dst: ring entry pos % window; state_row: slot * ring_entries + pos % ring_entries.
+ *                -1 where there is nothing to write, and where a later token of the row takes the same ring entry.
+ *   row values   n_compressed = entries(now), cmp_lengths = min(n_compressed, topk), swa_lengths = min(now, window), the window's pool
+ *                entries in the order of their positions (-1 behind them), block tables with zeros behind the pages held
+ *   token_starts the first token of each row, then their number; token values behind the last token are left as they were
+ *   lengths_out, free_counts_out  the state after the step: all slots, both counts.  Either may be the array it comes from.
+ * A row that cannot be served is left out: its tokens get position 0 and destinations -1, its row values are 0 / -1, its
+ * state stays.  That is a slot outside [0, capacity) (-1 is not reported) or one that an earlier row has (WUDA_DEV_BAD_SLOT), a
+ * negative length or token count, pages beyond table_width, tokens beyond max_tokens (WUDA_DEV_BAD_LENGTH), and a row that needs
+ * pages where the rows up to it need more than a stack holds (WUDA_DEV_NO_FREE_PAGE); rows behind it that need none are served.
+ *
+ * rows <= 4096, capacity <= 16384, max_tokens <= 262144, table_width <= 262144.
+ */
+typedef struct wuda_step_tables_args {
+    const int32_t* lengths;      /* int32 [capacity]: tokens that each slot's caches hold                */
+    int32_t* lengths_out;        /* int32 [capacity]                                                     */
+    int32_t* idx_table;          /* int32 [capacity, table_stride]: pages by slot, grown in place        */
+    int32_t* cmp_table;          /* int32 [capacity, table_stride]                                       */
+    const int32_t* swa_table;    /* int32 [capacity, ceil(window / swa_entries_per_block)]               */
+    const int32_t* idx_free;     /* int32 [free_capacity]: free pages, the next one last                 */
+    const int32_t* cmp_free;     /* int32 [free_capacity]                                                */
+    const int32_t* free_counts;  /* int32 [2]: idx, cmp                                                  */
+    int32_t* free_counts_out;    /* int32 [2]                                                            */
+    int64_t* pos;                /* int64 [max_tokens]                                                   */
+    int32_t* q_pos;              /* int32 [max_tokens]: the positions again                              */
+    int64_t* state_row;          /* int64 [max_tokens]                                                   */
+    int64_t* idx_dst;            /* int64 [max_tokens]                                                   */
+    int64_t* cmp_dst;            /* int64 [max_tokens]                                                   */
+    int64_t* swa_dst;            /* int64 [max_tokens]                                                   */
+    int32_t* token_starts;       /* int32 [rows + 1]                                                     */
+    int32_t* n_compressed;       /* int32 [rows]                                                         */
+    int32_t* cmp_lengths;        /* int32 [rows]                                                         */
+    int32_t* swa_lengths;        /* int32 [rows]                                                         */
+    int32_t* swa_indices;        /* int32 [rows, window]                                                 */
+    int32_t* idx_block_table;    /* int32 [rows, block_table_stride], table_width of them written        */
+    int32_t* cmp_block_table;    /* int32 [rows, block_table_stride]                                     */
+    int32_t* counter;            /* int32 [1], zero before the first call; a call leaves it at zero.  Calls that may overlap
+                                    on the device must not share it (nor the state).                     */
+    int64_t table_stride, block_table_stride;
+    int32_t capacity, table_width, idx_free_capacity, cmp_free_capacity, max_tokens;
+    int32_t idx_entries_per_block, cmp_entries_per_block, swa_entries_per_block, ratio, ring_entries, window, topk;
+} wuda_step_tables_args;
+int wuda_step_tables(const wuda_step_tables_args* args, const int32_t* slots, const int32_t* new_tokens, int rows,
+                     int32_t* status_word, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Beam selection: of all beams x vocabulary of a group, the k best continuations.
+ *
+ *   value[g, w, v] = scores[g, w] + logits[g, w, v] - log sum_u exp(logits[g, w, u])
+ * in descending order; equal values are resolved towards the lower beam, then the lower token.  The comparison is that of
+ * (score + logit) - log sum in 64 bits (within a beam: of the logits); sums of exponentials are held in 32 bits per thread and 64 across threads.
+ * A logit that is not finite (a masked token) takes no part, a score that is not finite ends its beam: it has no
+ * continuation.  A finished beam has one, (scores[g, w], eos_token); the logits of either are not read.
+ * Where a group has fewer than k continuations, the rest is (-inf, parent -1, token -1).
+ *   finished_out[g, j] = the parent is finished, or the token is eos_token
+ *
+ * groups <= 256, width <= 32, k <= 64, vocab <= 2^24.  The result does not depend on how the work is split among CTAs of one
+ * call of the same sizes, nor on the alignment of the rows: beams with the same logits get the same sums, bit for bit.
+ */
+typedef struct wuda_beam_select_args {
+    const void* logits;          /* [groups, width, vocab], the vocabulary contiguous                    */
+    int64_t group_stride, beam_stride; /* in elements                                                    */
+    const float* scores;         /* fp32 [groups, width]                                                 */
+    const uint8_t* finished;     /* [groups, width], nonzero = finished; nullable                        */
+    float* scores_out;           /* fp32 [groups, k]                                                     */
+    int32_t* parents_out;        /* int32 [groups, k]                                                    */
+    int32_t* tokens_out;         /* int32 [groups, k]                                                    */
+    uint8_t* finished_out;       /* [groups, k], 0 or 1                                                  */
+    void* workspace;             /* wuda_beam_select_workspace_bytes(...) bytes, 16-byte aligned          */
+    int64_t workspace_bytes;
+    int32_t* counters;           /* int32 [groups], zero before the first call; a call leaves them at zero */
+    int32_t groups, width, vocab, k, eos_token; /* eos_token -1: no token finishes a beam                 */
+    int32_t logits_type;         /* 0 bf16, 1 fp16, 2 fp32                                               */
+} wuda_beam_select_args;
+/* Bytes of workspace, or -1 on sizes that are refused. */
+int64_t wuda_beam_select_workspace_bytes(int groups, int width, int vocab, int k, int logits_type);
+int wuda_beam_select(const wuda_beam_select_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Beam reordering: after a selection, beam j of a group continues beam parents[g, j].  The first child of a beam keeps its
+ * request slot; every further child takes the slot of a beam without children (children and free slots in ascending order of
+ * their beams) and is a fork: what its parent's slot holds is copied to its own.  No memory is allocated: the slots of a group hold
+ * equally many tokens, share their pages up to shared_lengths and own the same number of pages behind them.
+ *
+ *   slots_out[g, j]  the slot of new beam j.  A beam without a parent (parents -1) gets a slot that is left over, its contents as
+ *                    they were; -1 where there is none
+ *   states           row `slot` of each array, row_bytes bytes
+ *   pools            per page: entries_per_block x segment_bytes[0], then entries_per_block x segment_bytes[1].  A slot holds
+ *                    lengths / tokens_per_entry entries through its row of `table`, or min(lengths, ring) where ring > 0.  Copied are
+ *                    those behind the shared pages: from page (shared_lengths / tokens_per_entry) / entries_per_block on (ring > 0: all).
+ * A slot outside [0, capacity) or given twice takes no part (-1 is not reported, else WUDA_DEV_BAD_SLOT); a parent without a
+ * slot counts as none, so does one outside [0, width) (-1 is not reported, else WUDA_DEV_BAD_PARENT); a fork between slots of different or
+ * negative lengths, or of more pages than the table has, is not made and its beam gets slot -1 (WUDA_DEV_BAD_LENGTH); a page
+ * outside the pool is not copied (WUDA_DEV_BAD_PAGE_INDEX).
+ *
+ * width <= 32, groups * width <= 4096, capacity <= 16384.  slots_out must not be slots.
+ */
+#define WUDA_BEAM_MAX_STATES 8
+#define WUDA_BEAM_MAX_POOLS 4
+typedef struct wuda_beam_state {
+    void* data;                  /* [capacity, row_bytes], 4-byte aligned                                 */
+    int64_t row_bytes;           /* a multiple of 4                                                      */
+} wuda_beam_state;
+typedef struct wuda_beam_pool {
+    void* data;                  /* uint8 [num_blocks, stride_bytes], 16-byte aligned                    */
+    const int32_t* table;        /* int32 [capacity, table_width]                                        */
+    int64_t stride_bytes;        /* a multiple of 16                                                     */
+    int32_t num_blocks, table_width, entries_per_block;
+    int32_t segment_bytes[2];    /* multiples of 4, the second may be 0; entries_per_block x the first is a multiple of 16 */
+    int32_t tokens_per_entry, ring;
+    int32_t reserved;
+} wuda_beam_pool;
+typedef struct wuda_beam_reorder_args {
+    const int32_t* lengths;      /* int32 [capacity]                                                     */
+    const int32_t* shared_lengths; /* int32 [capacity], nullable: nothing is shared                      */
+    wuda_beam_state states[WUDA_BEAM_MAX_STATES];
+    wuda_beam_pool pools[WUDA_BEAM_MAX_POOLS];
+    int32_t num_states, num_pools, capacity, width;
+} wuda_beam_reorder_args;
+int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32_t* parents, const int32_t* slots, int32_t* slots_out, int groups,
+                      int32_t* status_word, void* stream);
 
 #ifdef __cplusplus
 }

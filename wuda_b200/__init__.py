@@ -20,3 +20,5 @@ if not _running_the_build_module():
     from .ops import *  # noqa: F401,F403
     from .ops import _fast  # noqa: F401
     from .shims import *  # noqa: F401,F403
+    from .step_tables import StepTables  # noqa: F401
+    from .beams import BeamReorder, PagedState  # noqa: F401

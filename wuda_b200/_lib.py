@@ -113,6 +113,45 @@ class LayerStep(ctypes.Structure):
                  ("logits_stride", c_i64)])
 
 
+class StepTablesArgs(ctypes.Structure):
+    """wuda_step_tables_args"""
+    _fields_ = ([(n, c_vp) for n in ("lengths", "lengths_out", "idx_table", "cmp_table", "swa_table", "idx_free", "cmp_free",
+                                     "free_counts", "free_counts_out", "pos", "q_pos", "state_row", "idx_dst", "cmp_dst", "swa_dst",
+                                     "token_starts", "n_compressed", "cmp_lengths", "swa_lengths", "swa_indices",
+                                     "idx_block_table", "cmp_block_table", "counter")] +
+                [("table_stride", c_i64), ("block_table_stride", c_i64)] +
+                [(n, ctypes.c_int32) for n in ("capacity", "table_width", "idx_free_capacity", "cmp_free_capacity", "max_tokens",
+                                               "idx_entries_per_block", "cmp_entries_per_block", "swa_entries_per_block",
+                                               "ratio", "ring_entries", "window", "topk")])
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """wuda_beam_select_args"""
+    _fields_ = [("logits", c_vp), ("group_stride", c_i64), ("beam_stride", c_i64), ("scores", c_vp), ("finished", c_vp),
+                ("scores_out", c_vp), ("parents_out", c_vp), ("tokens_out", c_vp), ("finished_out", c_vp), ("workspace", c_vp),
+                ("workspace_bytes", c_i64), ("counters", c_vp), ("groups", ctypes.c_int32), ("width", ctypes.c_int32),
+                ("vocab", ctypes.c_int32), ("k", ctypes.c_int32), ("eos_token", ctypes.c_int32), ("logits_type", ctypes.c_int32)]
+
+
+class BeamState(ctypes.Structure):
+    """wuda_beam_state"""
+    _fields_ = [("data", c_vp), ("row_bytes", c_i64)]
+
+
+class BeamPool(ctypes.Structure):
+    """wuda_beam_pool"""
+    _fields_ = [("data", c_vp), ("table", c_vp), ("stride_bytes", c_i64), ("num_blocks", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("entries_per_block", ctypes.c_int32), ("segment_bytes", ctypes.c_int32 * 2),
+                ("tokens_per_entry", ctypes.c_int32), ("ring", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class BeamReorderArgs(ctypes.Structure):
+    """wuda_beam_reorder_args"""
+    _fields_ = [("lengths", c_vp), ("shared_lengths", c_vp), ("states", BeamState * 8), ("pools", BeamPool * 4),
+                ("num_states", ctypes.c_int32), ("num_pools", ctypes.c_int32), ("capacity", ctypes.c_int32),
+                ("width", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); mirrors include/wuda_b200.h one to one.
 SIGNATURES = {
     "wuda_version": (c_int, []),
@@ -191,6 +230,10 @@ SIGNATURES = {
     "wuda_layer_workspace_bytes": (c_i64, [ctypes.POINTER(LayerWeights), c_int, c_int, c_i64, c_int]),
     "wuda_layer_workspace_offset": (c_i64, [ctypes.POINTER(LayerWeights), c_int, c_int, c_i64, c_int, ctypes.c_char_p]),
     "wuda_layer_sm_shares": (c_int, [c_int, c_int, c_int, c_int, c_int, c_vp]),
+    "wuda_step_tables": (c_int, [ctypes.POINTER(StepTablesArgs), c_vp, c_vp, c_int, c_vp, c_vp]),
+    "wuda_beam_select_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int, c_int]),
+    "wuda_beam_select": (c_int, [ctypes.POINTER(BeamSelectArgs), c_vp]),
+    "wuda_beam_reorder": (c_int, [ctypes.POINTER(BeamReorderArgs), c_vp, c_vp, c_vp, c_int, c_vp, c_vp]),
     "wuda_layer_decode": (c_int, [ctypes.POINTER(LayerWeights), ctypes.POINTER(LayerState), ctypes.POINTER(LayerStep),
                                   c_int, c_vp]),
 }

@@ -1,0 +1,74 @@
+// The request slots of a batch in shared memory: which rows have one, and which row has it first.  Every CTA of a kernel finds
+// that out for itself (a few hundred cycles beside the loads that it waits for anyway), so that no launch is needed in front.
+#pragma once
+#include <climits>
+
+#include "host.h"
+
+namespace wuda {
+
+constexpr int kMostSlots = 16384;      // one word of shared memory per slot
+constexpr int kMostRows = 4096;
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void report(int32_t* status, int code) {
+    if (status) atomicCAS(status, 0, code);
+}
+
+// slot[b] = slots[b], or -1 where it is outside [0, capacity) or an earlier row has it.  `first`: capacity words, whatever they
+// hold.  All threads of the block; the rows of a thread are [b0, b1).  Ends behind a barrier.
+__device__ __forceinline__ void load_slots(const int32_t* __restrict__ slots, int b0, int b1, int capacity, int* slot, int* first,
+                                           int32_t* status) {
+    for (int b = b0; b < b1; ++b) {
+        const int s = slots[b];
+        const bool inside = s >= 0 && s < capacity;
+        if (!inside && s != -1) report(status, WUDA_DEV_BAD_SLOT);
+        slot[b] = inside ? s : -1;
+        if (inside) first[s] = INT_MAX;
+    }
+    __syncthreads();
+    for (int b = b0; b < b1; ++b)
+        if (slot[b] >= 0) atomicMin(&first[slot[b]], b);
+    __syncthreads();
+    for (int b = b0; b < b1; ++b)
+        if (slot[b] >= 0 && first[slot[b]] != b) {
+            report(status, WUDA_DEV_BAD_SLOT);
+            slot[b] = -1;
+        }
+}
+
+// Exclusive sums of N counts over the block's threads, in thread order, and the totals.  `scratch`: N * 33 words.
+template <int N, int THREADS>
+__device__ __forceinline__ void block_exclusive_sum(int (&v)[N], int (&total)[N], int* scratch) {
+    static_assert(THREADS % 32 == 0 && THREADS <= 1024, "whole warps");
+    constexpr int kWarps = THREADS / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inclusive[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        int x = v[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        inclusive[i] = x;
+        if (lane == 31) scratch[i * 33 + warp] = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        int x = lane < kWarps ? scratch[i * 33 + lane] : 0;      // every warp adds the warps' sums for itself
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        total[i] = __shfl_sync(0xffffffffu, x, 31);
+        const int before = __shfl_sync(0xffffffffu, x, warp == 0 ? 0 : warp - 1);
+        v[i] = inclusive[i] - v[i] + (warp == 0 ? 0 : before);
+    }
+}
+#endif
+
+}  // namespace wuda

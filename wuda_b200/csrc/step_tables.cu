@@ -1,0 +1,271 @@
+// Step tables: positions, cache destinations, block tables and window entries of a step from the lengths of its requests, with the
+// pages that growing requests take from the free stacks.
+//
+// For a row (slot, n tokens) with old = lengths[slot], now = old + n:  pages(x) = ceil((x / ratio) / entries_per_block) of each
+// compressed pool are held at length x, so a row takes need = pages(now) - pages(old) pages; with `first` the sum of the needs of the rows
+// in front of it, its page j >= pages(old) is free[count - 1 - (first + j - pages(old))].  Everything else follows from
+// positions, divisions and the page tables, token by token and column by column.
+//
+// One CTA works out the rows (slots, lengths, a scan over the needs) in shared memory, then its warps write the outputs.
+#include "batch_slots.cuh"
+
+namespace wuda {
+namespace steptables {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+
+struct Params {
+    wuda_step_tables_args a;
+    const int32_t* slots;
+    const int32_t* new_tokens;
+    int rows;
+    int32_t* status;
+};
+
+// What is known of a row, in shared memory
+struct Rows {
+    int* slot;        // -1: left out
+    int* old_len;
+    int* new_len;
+    int* idx_first;   // pages that the rows in front of it take
+    int* cmp_first;
+    int* start;       // rows + 1
+    int* first;       // (load_slots)
+    __device__ Rows(int* mem, int rows) {
+        slot = mem, old_len = slot + rows, new_len = old_len + rows, idx_first = new_len + rows, cmp_first = idx_first + rows;
+        start = cmp_first + rows, first = start + rows + 1;
+    }
+};
+inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (6ull * rows + 1 + capacity); }
+
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, int ratio, int epb) { return (tokens / ratio + epb - 1) / epb; }
+
+__device__ __forceinline__ int cut_count(int count, int capacity, int32_t* status) {
+    if (count >= 0 && count <= capacity) return count;
+    report(status, WUDA_DEV_BAD_LENGTH);
+    return count < 0 ? 0 : capacity;
+}
+
+// Page `page` of a row: held before, or taken from the free stack in this step.
+struct PoolView {
+    const int32_t* table;   // the slot's row
+    const int32_t* free;
+    int held, top;          // page `held` is free[top], the next one free[top - 1]
+    __device__ int operator()(int page) const { return page < held ? table[page] : free[top - (page - held)]; }
+};
+
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
+    extern __shared__ int mem[];
+    __shared__ int scan[3 * 33];
+    __shared__ int taken[2];
+    const wuda_step_tables_args& a = p.a;
+    const int rows = p.rows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Rows r(mem, rows);
+    pdl_launch_dependents();
+    pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
+    int32_t* status = p.status;
+
+    // ---- the rows
+    const int per = (rows + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, rows), b1 = min(b0 + per, rows);
+    load_slots(p.slots, b0, b1, a.capacity, r.slot, r.first, status);
+    const int free_idx = cut_count(a.free_counts[0], a.idx_free_capacity, status);
+    const int free_cmp = cut_count(a.free_counts[1], a.cmp_free_capacity, status);
+    int sum[3] = {0, 0, 0}, total[3];      // tokens, pages of both pools
+    for (int b = b0; b < b1; ++b) {
+        const int n = p.new_tokens ? p.new_tokens[b] : 1;
+        const int counted = min(max(n, 0), a.max_tokens + 1);
+        r.start[b] = sum[0];
+        sum[0] += counted;
+        const int slot = r.slot[b];
+        if (slot < 0) continue;
+        const int old = a.lengths[slot];
+        const int64_t now = static_cast<int64_t>(old) + n;
+        const int64_t idx_pages = pages_of(now, a.ratio, a.idx_entries_per_block), cmp_pages = pages_of(now, a.ratio, a.cmp_entries_per_block);
+        if (old < 0 || n < 0 || now > INT_MAX || idx_pages > a.table_width || cmp_pages > a.table_width) {
+            report(status, WUDA_DEV_BAD_LENGTH);
+            r.slot[b] = -1;
+            continue;
+        }
+        r.old_len[b] = old;
+        r.new_len[b] = static_cast<int>(now);
+        r.idx_first[b] = sum[1];
+        r.cmp_first[b] = sum[2];
+        sum[1] += static_cast<int>(idx_pages - pages_of(old, a.ratio, a.idx_entries_per_block));
+        sum[2] += static_cast<int>(cmp_pages - pages_of(old, a.ratio, a.cmp_entries_per_block));
+    }
+    block_exclusive_sum<3, kThreads>(sum, total, scan);
+    if (tid == 0) {
+        taken[0] = taken[1] = 0;
+        r.start[rows] = min(total[0], a.max_tokens);
+    }
+    __syncthreads();
+    // Rows that would reach beyond the buffers or the stacks.  Their needs are in the sums of the rows behind them, which is the rule:
+    // of the rows that need pages none behind the first that finds too few is served.  (Tokens beyond the buffers are a suffix, too.)
+    for (int b = b0; b < b1; ++b) {
+        const int n = max(p.new_tokens ? p.new_tokens[b] : 1, 0);
+        const int begin = r.start[b] + sum[0];
+        r.start[b] = min(begin, a.max_tokens);
+        if (r.slot[b] < 0) continue;
+        const int64_t old = r.old_len[b], now = r.new_len[b];
+        const int idx_first = r.idx_first[b] + sum[1], cmp_first = r.cmp_first[b] + sum[2];
+        const int idx_need = static_cast<int>(pages_of(now, a.ratio, a.idx_entries_per_block) - pages_of(old, a.ratio, a.idx_entries_per_block));
+        const int cmp_need = static_cast<int>(pages_of(now, a.ratio, a.cmp_entries_per_block) - pages_of(old, a.ratio, a.cmp_entries_per_block));
+        if (begin + static_cast<int64_t>(n) > a.max_tokens) {
+            report(status, WUDA_DEV_BAD_LENGTH);
+            r.slot[b] = -1;
+        } else if (idx_need + cmp_need > 0 && (idx_first + idx_need > free_idx || cmp_first + cmp_need > free_cmp)) {
+            report(status, WUDA_DEV_NO_FREE_PAGE);
+            r.slot[b] = -1;
+        } else {
+            r.idx_first[b] = free_idx - 1 - idx_first;      // (kept as the place of its first page in the stack)
+            r.cmp_first[b] = free_cmp - 1 - cmp_first;
+            if (idx_need + cmp_need > 0) {
+                atomicMax(&taken[0], idx_first + idx_need);
+                atomicMax(&taken[1], cmp_first + cmp_need);
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- block tables, 256 columns of one pool's row per warp
+    const int pieces = (a.table_width + 255) / 256;
+    const int tables = rows * 2 * pieces;
+    for (int task = warp; task < tables; task += kWarps) {
+        const int piece = task % pieces, of = task / pieces, b = of >> 1;
+        const bool cmp = of & 1;
+        const int epb = cmp ? a.cmp_entries_per_block : a.idx_entries_per_block;
+        const int slot = r.slot[b];
+        int32_t* out = (cmp ? a.cmp_block_table : a.idx_block_table) + b * a.block_table_stride;
+        PoolView pool = {};
+        int pages = 0;
+        int32_t* table = nullptr;
+        if (slot >= 0) {
+            table = (cmp ? a.cmp_table : a.idx_table) + slot * a.table_stride;
+            pages = static_cast<int>(pages_of(r.new_len[b], a.ratio, epb));
+            pool = {table, cmp ? a.cmp_free : a.idx_free, static_cast<int>(pages_of(r.old_len[b], a.ratio, epb)), cmp ? r.cmp_first[b] : r.idx_first[b]};
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int column = piece * 256 + i * 32 + lane;
+            if (column >= a.table_width) break;
+            const int page = column < pages ? pool(column) : 0;
+            out[column] = page;
+            if (column < pages && column >= pool.held) table[column] = page;
+        }
+    }
+
+    // ---- row values and window entries, a row per warp
+    const int window_pages = (a.window + a.swa_entries_per_block - 1) / a.swa_entries_per_block;
+    for (int b = warp; b < rows; b += kWarps) {
+        const int slot = r.slot[b], now = slot >= 0 ? r.new_len[b] : 0;
+        const int valid = min(now, a.window);
+        const int32_t* pages = a.swa_table + static_cast<int64_t>(max(slot, 0)) * window_pages;
+        for (int i = lane; i < a.window; i += 32) {
+            const int ring = i < valid ? (now - valid + i) % a.window : 0;
+            a.swa_indices[static_cast<int64_t>(b) * a.window + i] =
+                i < valid ? pages[ring / a.swa_entries_per_block] * a.swa_entries_per_block + ring % a.swa_entries_per_block : -1;
+        }
+        if (lane == 0) {
+            const int entries = now / a.ratio;
+            a.n_compressed[b] = entries;
+            a.cmp_lengths[b] = min(entries, a.topk);
+            a.swa_lengths[b] = valid;
+        }
+    }
+    for (int b = tid; b <= rows; b += kThreads) a.token_starts[b] = r.start[b];
+
+    // ---- tokens
+    const int tokens = r.start[rows];
+    for (int t = tid; t < tokens; t += kThreads) {
+        int b = 0;       // the last row that starts at or before t (rows without tokens start where the next one does)
+        for (int lo = 0, hi = rows; lo < hi;) {
+            const int mid = (lo + hi) >> 1;
+            if (r.start[mid] <= t) b = mid, lo = mid + 1;
+            else hi = mid;
+        }
+        const int slot = r.slot[b];
+        int pos = 0;
+        int64_t state = -1, idx = -1, cmp = -1, swa = -1;
+        if (slot >= 0) {
+            const int old = r.old_len[b], now = r.new_len[b];
+            pos = old + t - r.start[b];
+            if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + pos % a.ring_entries;
+            if (pos >= now - a.window) {
+                const int ring = pos % a.window;
+                swa = static_cast<int64_t>(a.swa_table[static_cast<int64_t>(slot) * window_pages + ring / a.swa_entries_per_block]) *
+                          a.swa_entries_per_block + ring % a.swa_entries_per_block;
+            }
+            if ((pos + 1u) % a.ratio == 0) {
+                const int entry = static_cast<int>((pos + 1u) / a.ratio) - 1;
+                const PoolView ip = {a.idx_table + slot * a.table_stride, a.idx_free, static_cast<int>(pages_of(old, a.ratio, a.idx_entries_per_block)),
+                                     r.idx_first[b]};
+                const PoolView cp = {a.cmp_table + slot * a.table_stride, a.cmp_free, static_cast<int>(pages_of(old, a.ratio, a.cmp_entries_per_block)),
+                                     r.cmp_first[b]};
+                idx = static_cast<int64_t>(ip(entry / a.idx_entries_per_block)) * a.idx_entries_per_block + entry % a.idx_entries_per_block;
+                cmp = static_cast<int64_t>(cp(entry / a.cmp_entries_per_block)) * a.cmp_entries_per_block + entry % a.cmp_entries_per_block;
+            }
+        }
+        a.pos[t] = pos;
+        a.q_pos[t] = pos;
+        a.state_row[t] = state;
+        a.idx_dst[t] = idx;
+        a.cmp_dst[t] = cmp;
+        a.swa_dst[t] = swa;
+    }
+
+    // ---- the state after the step
+    if (a.lengths_out != a.lengths) {
+        for (int s = tid; s < a.capacity; s += kThreads) a.lengths_out[s] = a.lengths[s];
+        __syncthreads();
+    }
+    for (int b = b0; b < b1; ++b)
+        if (r.slot[b] >= 0) a.lengths_out[r.slot[b]] = r.new_len[b];
+    if (tid == 0) {
+        a.free_counts_out[0] = free_idx - taken[0];
+        a.free_counts_out[1] = free_cmp - taken[1];
+    }
+}
+
+}  // namespace steptables
+}  // namespace wuda
+
+extern "C" int wuda_step_tables(const wuda_step_tables_args* args, const int32_t* slots, const int32_t* new_tokens, int rows,
+                                int32_t* status_word, void* stream) {
+    using namespace wuda;
+    using namespace wuda::steptables;
+    clear_error();
+    WUDA_REQUIRE(args, "args must not be NULL");
+    const wuda_step_tables_args& a = *args;
+    WUDA_REQUIRE(rows >= 0 && rows <= kMostRows, "rows must be in [0, %d] (got %d)", kMostRows, rows);
+    WUDA_REQUIRE(a.capacity >= 1 && a.capacity <= kMostSlots, "capacity must be in [1, %d] (got %d)", kMostSlots, a.capacity);
+    WUDA_REQUIRE(a.table_width >= 1 && a.table_width <= 262144, "table_width must be in [1, 262144] (got %d)", a.table_width);
+    WUDA_REQUIRE(a.max_tokens >= 0 && a.max_tokens <= 262144, "max_tokens must be in [0, 262144] (got %d)", a.max_tokens);
+    WUDA_REQUIRE(new_tokens || rows <= a.max_tokens, "%d rows of one token do not fit max_tokens = %d", rows, a.max_tokens);
+    WUDA_REQUIRE(a.table_stride >= a.table_width && a.block_table_stride >= a.table_width, "the tables' rows are shorter than table_width");
+    WUDA_REQUIRE(a.idx_free_capacity >= 0 && a.cmp_free_capacity >= 0, "a free stack of negative size");
+    WUDA_REQUIRE(a.idx_entries_per_block >= 1 && a.cmp_entries_per_block >= 1 && a.swa_entries_per_block >= 1,
+                 "entries per block must be positive");
+    WUDA_REQUIRE(a.ratio >= 1 && a.ring_entries >= 1 && a.window >= 1 && a.window <= 65536 && a.topk >= 0,
+                 "ratio, ring_entries and window must be positive, window at most 65536, topk not negative");
+    WUDA_REQUIRE(a.lengths && a.lengths_out && a.idx_table && a.cmp_table && a.swa_table && a.free_counts && a.free_counts_out &&
+                     a.token_starts && a.n_compressed && a.cmp_lengths && a.swa_lengths && a.swa_indices && a.idx_block_table &&
+                     a.cmp_block_table && a.counter,
+                 "state, row outputs and counter must not be NULL");
+    WUDA_REQUIRE(a.max_tokens == 0 || (a.pos && a.q_pos && a.state_row && a.idx_dst && a.cmp_dst && a.swa_dst),
+                 "token outputs must not be NULL");
+    WUDA_REQUIRE((a.idx_free || a.idx_free_capacity == 0) && (a.cmp_free || a.cmp_free_capacity == 0), "free stacks must not be NULL");
+    WUDA_REQUIRE(a.idx_table != a.cmp_table, "the two pools must not share a page table");
+    if (rows == 0) return WUDA_OK;
+    WUDA_REQUIRE(slots, "slots must not be NULL");
+    DeviceInfo dev;
+    if (const int st = current_device_info(&dev)) return st;
+    const size_t smem = shared_bytes(rows, a.capacity);
+    if (smem > 48 * 1024 - 1024)
+        WUDA_CUDA(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(shared_bytes(kMostRows, kMostSlots))));
+    Params p = {a, slots, new_tokens, rows, status_word};
+    WUDA_CUDA(launch_pdl(step_tables_kernel, dim3(1), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p));
+    return WUDA_OK;
+}

@@ -84,7 +84,8 @@ class KVCacheManager:
         for slot in range(capacity):
             self._reset_state(slot)
         self._free_slots = list(range(capacity - 1, -1, -1))
-        self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables}
+        self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables, "shared": tokens in shared pages}
+        self._owners = {"cmp": {}, "idx": {}}      # page -> requests that hold it, where they are more than one
 
     # ---- slot lifecycle: a new or reused slot starts with kv = 0, score = -inf
     def _reset_state(self, slot):
@@ -114,8 +115,55 @@ class KVCacheManager:
     def free_request(self, slot):
         req = self.reqs.pop(slot)
         for name in ("swa", "cmp", "idx"):
-            self._pools[name].give_back(req[name])
+            self._pools[name].give_back(self._given_up(name, req[name]))
         self._free_slots.append(slot)
+
+    def _given_up(self, name, pages):
+        """Those of a request's pages that no other request holds any longer."""
+        owners = self._owners.get(name)
+        if not owners:
+            return pages
+        last = []
+        for page in pages:
+            left = owners.get(page, 1) - 1
+            if left >= 2:
+                owners[page] = left
+            else:
+                owners.pop(page, None)
+            if left == 0:
+                last.append(page)
+        return last
+
+    def fork_request(self, slot, copies):
+        """`copies` new requests that continue request `slot` (the beams of a prompt; not in the reference's manager).  Returns
+        their slots.  All of them, the request included, share its filled compressed pages; state rings, window pages and
+        the compressed page that is being filled are copied.  A request that shares pages already is not forked again."""
+        req = self.reqs[slot]
+        if req.get("shared"):
+            raise ValueError("request %d shares its pages already" % slot)
+        entries = (req["pos"] + 1) // RATIO
+        own = {name: len(req[name]) - min(entries // self.entries_per_block[name], len(req[name])) for name in ("cmp", "idx")}
+        if copies < 0 or copies > len(self._free_slots) or any(
+                copies * n > len(self._pools[name]._free) for name, n in dict(own, swa=len(req["swa"])).items()):
+            raise ValueError("no room for %d more requests" % copies)
+        slots = []
+        for _ in range(copies):
+            new = self._free_slots.pop()
+            self.main_state[new] = self.main_state[slot]
+            self.idx_state[new] = self.idx_state[slot]
+            self.reqs[new] = {"pos": req["pos"], "shared": req["pos"] + 1}
+            for name, mine in dict(own, swa=len(req["swa"])).items():
+                pool, common = self._pools[name], len(req[name]) - mine
+                table = req[name][:common] + [pool.take() for _ in range(mine)]
+                for a, b in zip(req[name][common:], table[common:]):
+                    pool.data[b] = pool.data[a]
+                for page in table[:common]:
+                    self._owners[name][page] = self._owners[name].get(page, 1) + 1
+                self.reqs[new][name] = table
+            slots.append(new)
+        if copies:
+            req["shared"] = req["pos"] + 1
+        return slots
 
     # ---- one decode step: positions, state rows and cache destinations of every request
     def step_begin(self, slots):

@@ -32,6 +32,7 @@ import ctypes
 from . import _lib, moe, o_proj, ops
 from ._lib import check, lib
 from .decode import CsaDecodeStage
+from .step_tables import CacheTables
 
 WINDOW = 128
 
@@ -74,10 +75,31 @@ class AttentionHalfLayer:
         self.stage.q_raw = self.front_out[:, :csa_weights.q_lora]       # the chain reads the q_lora columns in place
         self.status = self.stage.status
         self.out = None
+        self.tables = None
         self._graph, self._graph_m, self._graph_x = None, 0, None
+
+    def device_tables(self):
+        """The cache's step tables on the device, filling this layer's step buffers (made by the first call, which takes over the
+        cache manager's present state; later changes there need tables.push())."""
+        if self.tables is None:
+            st = self.stage
+            st.idx_state_row = st.main_state_row       # (one ring geometry: the two rings' rows are the same)
+            self.tables = CacheTables(
+                self.cache, self.max_batch, topk=self.topk, status_word=self.status,
+                out=dict(pos=st.pos, q_pos=st.q_pos, state_row=st.main_state_row, idx_dst=st.idx_dst, cmp_dst=st.cmp_dst,
+                         swa_dst=st.swa_dst, n_compressed=st.n_compressed, cmp_lengths=self.cmp_len, swa_lengths=self.swa_len,
+                         swa_indices=self.swa_idx, idx_block_table=st.block_table, cmp_block_table=st.cmp_block_table))
+        return self.tables
+
+    def prepare_on_device(self, slots):
+        """prepare() without the host: slots int32 on the device, -1 for a padded row, whose residual streams get
+        through the layer without touching a cache."""
+        return self.device_tables().step(slots)
 
     def prepare(self, slots):
         """Host side of a step: positions, destinations, page tables, window entries (device copies only)."""
+        if self.tables is not None and self.tables.on_device:
+            raise _lib.WudaError(1, "the cache's step tables are on the device: prepare_on_device(), or pull() them first")
         st = self.stage.prepare(slots)
         m = len(slots)
         pos = st["pos"].tolist()
@@ -257,6 +279,12 @@ class DecoderLayer:
     def prepare(self, slots):
         return self.attn.prepare(slots)
 
+    def device_tables(self):
+        return self.attn.device_tables()
+
+    def prepare_on_device(self, slots):
+        return self.attn.prepare_on_device(slots)
+
     def launch_ffn(self, x, m):
         """The feed-forward half on the residual streams x bf16 [m, 4, hidden] (Python-sequenced form)."""
         f = self.ffn
@@ -276,15 +304,25 @@ class DecoderLayer:
             return self._launch_native(hidden_states, m)
         return self.launch_ffn(self.attn.launch(hidden_states, m), m)
 
-    def capture(self, hidden_states, m):
+    def capture(self, hidden_states, m, slots=None):
         """One eager pass, then the same pass as a CUDA graph reading `hidden_states` in place.  On a pair of
         ranks both must call this (and later replay()) the same number of times: the exchange steps number
-        their calls on the device."""
+        their calls on the device.  With slots (int32 [m] on the device) the graph prepares its step itself
+        (prepare_on_device), so that every replay is the next token; the eager pass is taken back."""
+        if slots is not None:
+            tables = self.device_tables()
+            before = tables.lengths.clone(), tables.free_counts.clone()
+            self.prepare_on_device(slots)
         self.launch(hidden_states, m)
         torch.cuda.synchronize()
         self.check_status()
+        if slots is not None:      # (the pages it took are the ones that the first replay takes, and what it wrote is written again)
+            tables.lengths.copy_(before[0])
+            tables.free_counts.copy_(before[1])
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
+            if slots is not None:
+                self.prepare_on_device(slots)
             out = self.launch(hidden_states, m)
         self._graph, self._graph_out = graph, out
         return graph

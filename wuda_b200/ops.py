@@ -13,13 +13,13 @@ import torch
 
 from . import _lib, native_calls
 from ._lib import WudaError, check, lib
-from .scratch import Scratch
+from .scratch import FLAG_BYTES, Scratch
 
 __all__ = ["mqa_logits_fp4_decode_out", "mqa_logits_fp4_decode", "mqa_logits_fp8_decode_out", "fp8_paged_mqa_logits", "topk_v2", "topk_v2_transform",
            "IndexerHostPlan", "sparse_mla_decode", "flash_mla_with_kvcache", "device_status_word", "num_sms", "rmsnorm_quant", "act_quant", "rope_quant",
            "rmsnorm_rope_out", "mhc_post_out", "mhc_pre", "moe_gate", "bf16_gemm", "front_mixed_gemm", "idx_postprocess_fp8", "idx_postprocess", "cache_writers_fp8", "cache_writers_fp4", "mqa_compressor_fp8_standalone", "fp8_gemm", "TP2Link", "exchange_handles", "nvfp4_gemm",
            "fp4_gemm", "fp4_act_quant", "hc_split_sinkhorn", "head_ssq_standalone", "idx_postprocess_standalone",
-           "idx_postprocess_fp8_standalone", "mqa_compressor_standalone", "mqa_compressor_paged", "topk_v2_plan"]
+           "idx_postprocess_fp8_standalone", "mqa_compressor_standalone", "mqa_compressor_paged", "topk_v2_plan", "beam_select"]
 
 # The operators that a server calls by themselves try csrc/fast_ops.cpp first: checks, outputs and launch in one native call,
 # which does nothing and returns None for whatever it does not know or would have to refuse.
@@ -210,6 +210,53 @@ def topk_v2(scores, seq_lens, page_table, topk, page_size=64, raw_indices=None, 
     out = scores.new_empty((scores.size(0), int(topk)), dtype=torch.int32)
     return topk_v2_transform(scores, seq_lens, page_table, out, page_size, None, raw_indices,
                              rows_per_table_row=rows_per_table_row)
+
+
+_LOGITS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_beam_scratch = Scratch(zeroed=True)     # the groups' counters, then the CTAs' lists and sums
+
+
+def _on_current_device(t):
+    return t.is_cuda and t.device.index == torch._C._cuda_getDevice()
+
+
+def beam_select(logits, scores, k=None, *, finished=None, eos_token=None):
+    """The k best continuations of every group of beams over beams x vocabulary (no counterpart in the reference,
+    whose sampling is a host loop).
+
+    logits [groups, width, vocab] bf16, fp16 or fp32 with the vocabulary contiguous (any other strides), scores fp32
+    [groups, width] the beams' sums of log-probabilities; k defaults to width.  Returns
+      scores   fp32  [groups, k]  scores[g, parent] + log_softmax(logits[g, parent])[token], descending
+      parents  int32 [groups, k]  beam that the continuation belongs to
+      tokens   int32 [groups, k]
+      finished bool  [groups, k]  the parent is finished, or the token is eos_token
+    Equal values go to the lower beam, then the lower token.  Logits that are not finite take no part (masked tokens), a
+    beam whose score is not finite has no continuation, a finished beam (finished bool [groups, width], with an
+    eos_token) only itself with eos_token; the logits of both are not read.  Where fewer than k continuations are left, the rest is
+    (-inf, -1, -1, False).  groups <= 256, width <= 32, k <= 64."""
+    _require(logits.dim() == 3 and logits.dtype in _LOGITS_TYPES and _on_current_device(logits) and
+             (logits.stride(2) == 1 or logits.size(2) == 1),
+             "logits must be bf16, fp16 or fp32 [groups, width, vocab] on the current CUDA device with unit inner stride")
+    groups, width, vocab = logits.shape
+    _require(scores.device == logits.device and scores.dtype == torch.float32 and scores.is_contiguous() and
+             tuple(scores.shape) == (groups, width), "scores must be contiguous fp32 [groups, width] on the logits' device")
+    if finished is not None:
+        _require(finished.device == logits.device and finished.dtype == torch.bool and finished.is_contiguous() and
+                 tuple(finished.shape) == (groups, width), "finished must be contiguous bool [groups, width] on the logits' device")
+        _require(eos_token is not None, "finished beams need an eos_token")
+    k = width if k is None else int(k)
+    need = lib.wuda_beam_select_workspace_bytes(groups, width, vocab, k, _LOGITS_TYPES[logits.dtype])
+    _require(need >= 0, "beam_select: groups <= 256, width in [1, 32], vocab in [1, 2^24] and k in [1, 64] are implemented")
+    out = (scores.new_empty((groups, k)), scores.new_empty((groups, k), dtype=torch.int32),
+           scores.new_empty((groups, k), dtype=torch.int32), scores.new_empty((groups, k), dtype=torch.bool))
+    stream = _stream()
+    at, nbytes, flags, _hold = _beam_scratch.get(logits.device, stream, need + FLAG_BYTES)
+    a = _lib.BeamSelectArgs(logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), _ptr(finished),
+                            out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), at + FLAG_BYTES,
+                            nbytes - FLAG_BYTES, flags if flags is not None else at, groups, width, vocab, k,
+                            -1 if eos_token is None else int(eos_token), _LOGITS_TYPES[logits.dtype])
+    check(lib.wuda_beam_select(ctypes.byref(a), stream))
+    return out
 
 
 class IndexerHostPlan:
