@@ -6,7 +6,7 @@
 // in front of it, its page j >= pages(old) is free[count - 1 - (first + j - pages(old))].  Everything else follows from
 // positions, divisions and the page tables, token by token and column by column.
 //
-// One CTA works out the rows (slots, lengths, a scan over the needs) in shared memory, then its warps write the outputs.
+// Every CTA works out all rows (slots, lengths, a scan over the needs) in shared memory, then the warps of all CTAs write the outputs.
 #include "batch_slots.cuh"
 
 namespace wuda {
@@ -14,6 +14,7 @@ namespace steptables {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kPiece = 256;      // columns of a block table that a warp writes at a time
 
 struct Params {
     wuda_step_tables_args a;
@@ -59,12 +60,13 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
     extern __shared__ int mem[];
     __shared__ int scan[3 * 33];
     __shared__ int taken[2];
+    __shared__ bool last;
     const wuda_step_tables_args& a = p.a;
     const int rows = p.rows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Rows r(mem, rows);
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
-    int32_t* status = p.status;
+    int32_t* status = blockIdx.x == 0 ? p.status : nullptr;
 
     // ---- the rows
     const int per = (rows + kThreads - 1) / kThreads;
@@ -129,102 +131,114 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
     }
     __syncthreads();
 
-    // ---- block tables, 256 columns of one pool's row per warp
-    const int pieces = (a.table_width + 255) / 256;
-    const int tables = rows * 2 * pieces;
-    for (int task = warp; task < tables; task += kWarps) {
-        const int piece = task % pieces, of = task / pieces, b = of >> 1;
-        const bool cmp = of & 1;
-        const int epb = cmp ? a.cmp_entries_per_block : a.idx_entries_per_block;
-        const int slot = r.slot[b];
-        int32_t* out = (cmp ? a.cmp_block_table : a.idx_block_table) + b * a.block_table_stride;
-        PoolView pool = {};
-        int pages = 0;
-        int32_t* table = nullptr;
-        if (slot >= 0) {
-            table = (cmp ? a.cmp_table : a.idx_table) + slot * a.table_stride;
-            pages = static_cast<int>(pages_of(r.new_len[b], a.ratio, epb));
-            pool = {table, cmp ? a.cmp_free : a.idx_free, static_cast<int>(pages_of(r.old_len[b], a.ratio, epb)), cmp ? r.cmp_first[b] : r.idx_first[b]};
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int column = piece * 256 + i * 32 + lane;
-            if (column >= a.table_width) break;
-            const int page = column < pages ? pool(column) : 0;
-            out[column] = page;
-            if (column < pages && column >= pool.held) table[column] = page;
-        }
-    }
-
-    // ---- row values and window entries, a row per warp
-    const int window_pages = (a.window + a.swa_entries_per_block - 1) / a.swa_entries_per_block;
-    for (int b = warp; b < rows; b += kWarps) {
-        const int slot = r.slot[b], now = slot >= 0 ? r.new_len[b] : 0;
-        const int valid = min(now, a.window);
-        const int32_t* pages = a.swa_table + static_cast<int64_t>(max(slot, 0)) * window_pages;
-        for (int i = lane; i < a.window; i += 32) {
-            const int ring = i < valid ? (now - valid + i) % a.window : 0;
-            a.swa_indices[static_cast<int64_t>(b) * a.window + i] =
-                i < valid ? pages[ring / a.swa_entries_per_block] * a.swa_entries_per_block + ring % a.swa_entries_per_block : -1;
-        }
-        if (lane == 0) {
-            const int entries = now / a.ratio;
-            a.n_compressed[b] = entries;
-            a.cmp_lengths[b] = min(entries, a.topk);
-            a.swa_lengths[b] = valid;
-        }
-    }
-    for (int b = tid; b <= rows; b += kThreads) a.token_starts[b] = r.start[b];
-
-    // ---- tokens
-    const int tokens = r.start[rows];
-    for (int t = tid; t < tokens; t += kThreads) {
-        int b = 0;       // the last row that starts at or before t (rows without tokens start where the next one does)
-        for (int lo = 0, hi = rows; lo < hi;) {
-            const int mid = (lo + hi) >> 1;
-            if (r.start[mid] <= t) b = mid, lo = mid + 1;
-            else hi = mid;
-        }
-        const int slot = r.slot[b];
-        int pos = 0;
-        int64_t state = -1, idx = -1, cmp = -1, swa = -1;
-        if (slot >= 0) {
-            const int old = r.old_len[b], now = r.new_len[b];
-            pos = old + t - r.start[b];
-            if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + pos % a.ring_entries;
-            if (pos >= now - a.window) {
-                const int ring = pos % a.window;
-                swa = static_cast<int64_t>(a.swa_table[static_cast<int64_t>(slot) * window_pages + ring / a.swa_entries_per_block]) *
-                          a.swa_entries_per_block + ring % a.swa_entries_per_block;
-            }
-            if ((pos + 1u) % a.ratio == 0) {
-                const int entry = static_cast<int>((pos + 1u) / a.ratio) - 1;
-                const PoolView ip = {a.idx_table + slot * a.table_stride, a.idx_free, static_cast<int>(pages_of(old, a.ratio, a.idx_entries_per_block)),
-                                     r.idx_first[b]};
-                const PoolView cp = {a.cmp_table + slot * a.table_stride, a.cmp_free, static_cast<int>(pages_of(old, a.ratio, a.cmp_entries_per_block)),
-                                     r.cmp_first[b]};
-                idx = static_cast<int64_t>(ip(entry / a.idx_entries_per_block)) * a.idx_entries_per_block + entry % a.idx_entries_per_block;
-                cmp = static_cast<int64_t>(cp(entry / a.cmp_entries_per_block)) * a.cmp_entries_per_block + entry % a.cmp_entries_per_block;
-            }
-        }
-        a.pos[t] = pos;
-        a.q_pos[t] = pos;
-        a.state_row[t] = state;
-        a.idx_dst[t] = idx;
-        a.cmp_dst[t] = cmp;
-        a.swa_dst[t] = swa;
-    }
-
-    // ---- the state after the step
-    if (a.lengths_out != a.lengths) {
-        for (int s = tid; s < a.capacity; s += kThreads) a.lengths_out[s] = a.lengths[s];
+    // ---- the state after the step.  In place it is written by the CTA that comes last here, when every CTA has read it.
+    const bool in_place = a.lengths_out == a.lengths || a.free_counts_out == a.free_counts;
+    bool mine = blockIdx.x == 0;
+    if (in_place && gridDim.x > 1) {
+        if (tid == 0) last = atomicInc(reinterpret_cast<unsigned*>(a.counter), gridDim.x - 1) == gridDim.x - 1;   // (wraps back to zero)
         __syncthreads();
+        mine = last;
     }
-    for (int b = b0; b < b1; ++b)
-        if (r.slot[b] >= 0) a.lengths_out[r.slot[b]] = r.new_len[b];
-    if (tid == 0) {
-        a.free_counts_out[0] = free_idx - taken[0];
-        a.free_counts_out[1] = free_cmp - taken[1];
+    if (mine) {
+        if (a.lengths_out != a.lengths) {
+            for (int s = tid; s < a.capacity; s += kThreads) a.lengths_out[s] = a.lengths[s];
+            __syncthreads();
+        }
+        for (int b = b0; b < b1; ++b)
+            if (r.slot[b] >= 0) a.lengths_out[r.slot[b]] = r.new_len[b];
+        if (tid == 0) {
+            a.free_counts_out[0] = free_idx - taken[0];
+            a.free_counts_out[1] = free_cmp - taken[1];
+        }
+    }
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= rows; b += kThreads) a.token_starts[b] = r.start[b];
+
+    // ---- the outputs, a task per warp: 256 columns of one pool's block table, a row's values and window entries, or 32 tokens
+    const int window_pages = (a.window + a.swa_entries_per_block - 1) / a.swa_entries_per_block;
+    const int tokens = r.start[rows];
+    const int pieces = (a.table_width + kPiece - 1) / kPiece, tables = rows * 2 * pieces;
+    const int tasks = tables + rows + (tokens + 31) / 32;
+    for (int task = blockIdx.x * kWarps + warp; task < tasks; task += gridDim.x * kWarps) {
+        if (task < tables) {
+            const int piece = task % pieces, of = task / pieces, b = of >> 1;
+            const bool cmp = of & 1;
+            const int epb = cmp ? a.cmp_entries_per_block : a.idx_entries_per_block;
+            const int slot = r.slot[b];
+            int32_t* out = (cmp ? a.cmp_block_table : a.idx_block_table) + b * a.block_table_stride;
+            PoolView pool = {};
+            int pages = 0;
+            int32_t* table = nullptr;
+            if (slot >= 0) {
+                table = (cmp ? a.cmp_table : a.idx_table) + slot * a.table_stride;
+                pages = static_cast<int>(pages_of(r.new_len[b], a.ratio, epb));
+                pool = {table, cmp ? a.cmp_free : a.idx_free, static_cast<int>(pages_of(r.old_len[b], a.ratio, epb)),
+                        cmp ? r.cmp_first[b] : r.idx_first[b]};
+            }
+            int page[kPiece / 32];
+#pragma unroll
+            for (int i = 0; i < kPiece / 32; ++i) {      // all loads, then all stores
+                const int column = piece * kPiece + i * 32 + lane;
+                page[i] = column < pages ? pool(column) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kPiece / 32; ++i) {
+                const int column = piece * kPiece + i * 32 + lane;
+                if (column < a.table_width) out[column] = page[i];
+                if (column < pages && column >= pool.held) table[column] = page[i];
+            }
+        } else if (task < tables + rows) {
+            const int b = task - tables;
+            const int slot = r.slot[b], now = slot >= 0 ? r.new_len[b] : 0;
+            const int valid = min(now, a.window);
+            const int32_t* pages = a.swa_table + static_cast<int64_t>(max(slot, 0)) * window_pages;
+            for (int i = lane; i < a.window; i += 32) {
+                const int ring = i < valid ? (now - valid + i) % a.window : 0;
+                a.swa_indices[static_cast<int64_t>(b) * a.window + i] =
+                    i < valid ? pages[ring / a.swa_entries_per_block] * a.swa_entries_per_block + ring % a.swa_entries_per_block : -1;
+            }
+            if (lane == 0) {
+                const int entries = now / a.ratio;
+                a.n_compressed[b] = entries;
+                a.cmp_lengths[b] = min(entries, a.topk);
+                a.swa_lengths[b] = valid;
+            }
+        } else if (const int t = (task - tables - rows) * 32 + lane; t < tokens) {
+            int b = 0;       // the last row that starts at or before t (rows without tokens start where the next one does)
+            for (int lo = 0, hi = rows; lo < hi;) {
+                const int mid = (lo + hi) >> 1;
+                if (r.start[mid] <= t) b = mid, lo = mid + 1;
+                else hi = mid;
+            }
+            const int slot = r.slot[b];
+            int pos = 0;
+            int64_t state = -1, idx = -1, cmp = -1, swa = -1;
+            if (slot >= 0) {
+                const int old = r.old_len[b], now = r.new_len[b];
+                pos = old + t - r.start[b];
+                if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + pos % a.ring_entries;
+                if (pos >= now - a.window) {
+                    const int ring = pos % a.window;
+                    swa = static_cast<int64_t>(a.swa_table[static_cast<int64_t>(slot) * window_pages + ring / a.swa_entries_per_block]) *
+                              a.swa_entries_per_block + ring % a.swa_entries_per_block;
+                }
+                if ((pos + 1u) % a.ratio == 0) {
+                    const int entry = static_cast<int>((pos + 1u) / a.ratio) - 1;
+                    const PoolView ip = {a.idx_table + slot * a.table_stride, a.idx_free,
+                                         static_cast<int>(pages_of(old, a.ratio, a.idx_entries_per_block)), r.idx_first[b]};
+                    const PoolView cp = {a.cmp_table + slot * a.table_stride, a.cmp_free,
+                                         static_cast<int>(pages_of(old, a.ratio, a.cmp_entries_per_block)), r.cmp_first[b]};
+                    idx = static_cast<int64_t>(ip(entry / a.idx_entries_per_block)) * a.idx_entries_per_block + entry % a.idx_entries_per_block;
+                    cmp = static_cast<int64_t>(cp(entry / a.cmp_entries_per_block)) * a.cmp_entries_per_block + entry % a.cmp_entries_per_block;
+                }
+            }
+            a.pos[t] = pos;
+            a.q_pos[t] = pos;
+            a.state_row[t] = state;
+            a.idx_dst[t] = idx;
+            a.cmp_dst[t] = cmp;
+            a.swa_dst[t] = swa;
+        }
     }
 }
 
@@ -266,6 +280,9 @@ extern "C" int wuda_step_tables(const wuda_step_tables_args* args, const int32_t
         WUDA_CUDA(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(shared_bytes(kMostRows, kMostSlots))));
     Params p = {a, slots, new_tokens, rows, status_word};
-    WUDA_CUDA(launch_pdl(step_tables_kernel, dim3(1), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p));
+    const int64_t tokens = new_tokens ? a.max_tokens : rows;
+    const int64_t tasks = static_cast<int64_t>(rows) * (2 * ((a.table_width + kPiece - 1) / kPiece) + 1) + (tokens + 31) / 32;
+    const int grid = static_cast<int>(tasks < static_cast<int64_t>(dev.num_sms) * kWarps ? (tasks + kWarps - 1) / kWarps : dev.num_sms);
+    WUDA_CUDA(launch_pdl(step_tables_kernel, dim3(grid), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }
