@@ -6,9 +6,24 @@
 // token): keys of (order-preserving logit, ~token) are unique, and the largest key is the first candidate.  Only candidates of
 // different beams are compared by value, in 64 bits.
 //
-// One CTA per beam finds maximum, sum and its k largest keys, one after the other; one CTA per group merges the beams' lists.
+// One launch.  A row of logits is cut into chunks, a CTA each, that are read once: 16 bytes per load, four loads per thread ahead of the
+// four that it works on.  Every thread keeps a reference r and the sum of exp(x - r) of its elements (r follows the maximum only
+// where a term would pass e^40: a rescaling is rare, and no term overflows).  Which element a thread gets depends on the element's number
+// alone, not on the row's alignment, so equal rows have equal sums.
+//
+// Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the first tile is a lower bound of the row's k-th
+// largest logit; only what passes it (a handful per tile) goes to a list in shared memory.  A tile that overflows the list (sorted rows,
+// rows of one value) ends in an exact selection over list and tile, which leaves the k largest and a new bound.
+//
+// The CTA that completes a group's counter merges its lists: the k-th largest of the lists' first candidates bounds what can be among
+// the k best, and the few that pass are ranked by counting.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <type_traits>
 
 #include "host.h"
 
@@ -17,17 +32,48 @@ namespace beams {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kVectors = 4;                 // 16-byte loads per thread and tile
 constexpr int kMostK = 64, kMostWidth = 32, kMostGroups = 256;
+constexpr int kList = 2048;                 // candidates that a CTA holds, and that a group's chunks may have together
+constexpr int kMostChunks = 64;
+constexpr int kCtas = 1184;                 // CTAs of a launch: eight per SM, taken as SMs come free
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
+
+using Key = unsigned long long;             // (ordered logit, ~token): unique, larger is better; 0 is none
+
+struct Partial {
+    double sum;                             // of exp(x - ref) over a chunk
+    float ref;
+    float unused;
+};
 
 struct Params {
     wuda_beam_select_args a;
-    unsigned long long* lists;      // [groups * width, k] keys in descending order, 0 behind them
-    double* lse;                    // [groups * width]
+    Key* lists;                             // [groups * width, chunks, k] in descending order, 0 behind them
+    Partial* partials;                      // [groups * width, chunks]
+    int chunks, chunk_vectors;              // vectors of 16 bytes per chunk, a multiple of the block's threads
 };
 
-__device__ __forceinline__ float value_of(float x) { return x; }
-__device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
-__device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+struct Type;
+template <>
+struct Type<float> {
+    static constexpr int kVec = 4;
+    static constexpr uint32_t kMasked = 0xff800000u;
+};
+template <>
+struct Type<__half> {
+    static constexpr int kVec = 8;
+    static constexpr uint32_t kMasked = 0xfc00fc00u;
+    using Pair = __half2;
+};
+template <>
+struct Type<__nv_bfloat16> {
+    static constexpr int kVec = 8;
+    static constexpr uint32_t kMasked = 0xff80ff80u;
+    using Pair = __nv_bfloat162;
+};
 
 // a word that grows with x (no NaN); 0 is below every number
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -35,109 +81,467 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+__device__ __forceinline__ Key key_of(float x, uint32_t token) { return (static_cast<Key>(ordered(x)) << 32) | ~token; }
+__device__ __forceinline__ uint32_t token_of(Key k) { return ~static_cast<uint32_t>(k); }
 
-template <typename T>
-__device__ __forceinline__ float finite_or_lowest(T raw) {      // a masked token is -inf
-    const float x = value_of(raw);
-    return fabsf(x) < INFINITY ? x : -INFINITY;
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_rows_kernel(const Params p) {
-    __shared__ float red_max[kWarps];
-    __shared__ double red_sum[kWarps];
-    __shared__ unsigned long long red_key[kWarps];
-    const wuda_beam_select_args& a = p.a;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (!(fabsf(a.scores[row]) < INFINITY) || (a.finished && a.finished[row])) return;
-    const T* x = static_cast<const T*>(a.logits) + (row / a.width) * a.group_stride + (row % a.width) * a.beam_stride;
-    float m = -INFINITY;
-    for (int i = tid; i < a.vocab; i += kThreads) m = fmaxf(m, finite_or_lowest(x[i]));
+// ---- a vector: 16 bytes of a row as four words
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// Elements [at, at + kVec) of a row; masked from `end` on.  ALIGNED: the row lies on 16 bytes.  Otherwise two aligned loads, both within
+// the row [0, vocab), are shifted together.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_vector(const T* __restrict__ row, int at, int end, int vocab) {
+    constexpr int kVec = Type<T>::kVec;
+    const T* p = row + at;
+    if (at + kVec <= end) {
+        if (ALIGNED) return load16(p);
+        const uintptr_t address = reinterpret_cast<uintptr_t>(p);
+        const int off = static_cast<int>(address & 15);
+        const T* low = reinterpret_cast<const T*>(address - off);
+        if (off == 0) return load16(p);
+        if (low >= row && low + 2 * kVec <= row + vocab) {
+            const uint4 a = load16(low), b = load16(low + kVec);
+            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (off & 8) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) red_max[warp] = m;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, red_max[i]);
-    float s = 0.f;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-        const float v = finite_or_lowest(x[i]);
-        if (v > -INFINITY) s += expf(v - m);
-    }
-    double d = s;
+                for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+            }
+            if (off & 4) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) red_sum[warp] = d;
-    __syncthreads();
-    if (tid == 0) {
-        double total = 0;
-        for (int i = 0; i < kWarps; ++i) total += red_sum[i];
-        p.lse[row] = m > -INFINITY ? static_cast<double>(m) + log(total) : 0.0;
-    }
-    unsigned long long below = ~0ull;
-    for (int j = 0; j < a.k; ++j) {
-        unsigned long long best = 0;
-        for (int i = tid; i < a.vocab; i += kThreads) {
-            const float v = finite_or_lowest(x[i]);
-            const unsigned long long key = v > -INFINITY ? (static_cast<unsigned long long>(ordered(v)) << 32) | ~static_cast<uint32_t>(i) : 0;
-            if (key < below && key > best) best = key;
+                for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+            }
+            const int bits = (off & 3) * 8;
+            return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                              __funnelshift_r(w[3], w[4], bits));
         }
+    }
+    uint32_t w[4] = {Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked};
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane == 0) red_key[warp] = best;
-        __syncthreads();
-        for (int i = 0; i < kWarps; ++i) best = max(best, red_key[i]);
-        if (tid == 0) p.lists[static_cast<int64_t>(row) * a.k + j] = best;
-        below = best;
-        __syncthreads();
+        for (int i = 0; i < 4; ++i)
+            if (at + i < end) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (at + i < end) {
+                const uint32_t x = reinterpret_cast<const uint16_t*>(p)[i];
+                w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (x << 16) : (w[i / 2] & 0xffff0000u) | x;
+            }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// NaN -> -inf in all elements of a word, and a word's elements as fp32
+template <typename T>
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+        return __float_as_uint(fmaxf(__uint_as_float(w), -INFINITY));
+    } else {
+        using Pair = typename Type<T>::Pair;
+        const uint32_t masked = Type<T>::kMasked;
+        const Pair m = __hmax2(*reinterpret_cast<const Pair*>(&w), *reinterpret_cast<const Pair*>(&masked));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_words(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else {
+        using Pair = typename Type<T>::Pair;
+        const Pair m = __hmax2(*reinterpret_cast<const Pair*>(&a), *reinterpret_cast<const Pair*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit type
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w), -INFINITY);
+    else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// element e of a tile's 16 words
+template <typename T>
+__device__ __forceinline__ float element(const uint32_t (&w)[4 * kVectors], int e) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+    else {
+        const float2 f = pair_of<T>(w[e / 2]);
+        return e & 1 ? f.y : f.x;
     }
 }
 
-// Position of each entry among all: how many come before it in (value descending, beam, logit descending, token).
-__global__ void __launch_bounds__(kThreads) beam_merge_kernel(const Params p) {
-    __shared__ double value[kMostWidth * kMostK];
+struct Shared {
+    Key list[kList];
+    int count;                              // candidates pushed (those beyond kList are lost)
+    float bound;                            // the k-th largest logit so far, or less
+    float part_max[128];                    // maxima of parts of a tile
+    int hits[2];
+    float warp_ref[kWarps];
+    double warp_sum[kWarps];
+    bool last;
+    // merging
+    double value[kList];
+    uint16_t passed[kList];
+    double lse[kMostWidth], score[kMostWidth];
+    int kind[kMostWidth];
+    double least;
+    int survivors, there;
+};
+
+__device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
+    const int n = __reduce_add_sync(0xffffffffu, mine);
+    if ((threadIdx.x & 31) == 0 && n) atomicAdd(&hits[turn], n);
+    __syncthreads();
+    const int total = hits[turn];
+    if (threadIdx.x == 0) hits[turn ^ 1] = 0;      // (the other one was read before this barrier)
+    __syncthreads();
+    return total;
+}
+
+// The k largest of the list's entries of tokens below `first_token` and the tile's elements, exactly: the largest K such that k keys are at
+// or above it, bit by bit.  They become the list.  All threads; ends behind a barrier.
+template <typename T>
+__device__ __noinline__ void select_exactly(Shared& sh, const uint32_t (&w)[4 * kVectors], int vec0, int c0, int tile_base, int k) {
+    constexpr int kVec = Type<T>::kVec;
+    Key held[kList / kThreads];
+    const int count = min(sh.count, kList);
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) {
+        const int at = i * kThreads + threadIdx.x;
+        held[i] = at < count && token_of(sh.list[at]) < static_cast<uint32_t>(tile_base) ? sh.list[at] : 0;
+    }
+    if (threadIdx.x == 0) sh.hits[0] = sh.hits[1] = 0;
+    __syncthreads();
+    const auto tile_key = [&](int u, int e) -> Key {
+        const float x = element<T>(w, u * kVec + e);
+        return x > -INFINITY ? key_of(x, static_cast<uint32_t>(c0 + (vec0 + u * kThreads) * kVec + e)) : 0;
+    };
+    Key least = 0;
+    for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
+        const Key want = least | (1ull << bit);
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < kList / kThreads; ++i) mine += held[i] >= want;
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) mine += tile_key(u, e) >= want;
+        const int total = block_total(mine, sh.hits, turn);
+        if (total >= k) least = want;
+        if (total == k) break;
+    }
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    const auto keep = [&](Key key) {
+        if (key != 0 && key >= least) sh.list[atomicAdd(&sh.count, 1)] = key;      // (k of them at most)
+    };
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) keep(held[i]);
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) keep(tile_key(u, e));
+    __syncthreads();
+    if (threadIdx.x == 0 && sh.count == k) sh.bound = unordered(static_cast<uint32_t>(least >> 32));
+    __syncthreads();
+}
+
+// A chunk of a row: its partial sum, and its k largest keys in descending order.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row, int row_number, int number) {
+    constexpr int kVec = Type<T>::kVec, kWords = 4 * kVectors;
     const wuda_beam_select_args& a = p.a;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int g = blockIdx.x, tid = threadIdx.x, entries = a.width * a.k;
-    int there = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
+    const int c0 = number * p.chunk_vectors * kVec, end = min(a.vocab, c0 + p.chunk_vectors * kVec);
+    if (tid == 0) {
+        sh.count = 0;
+        sh.bound = -INFINITY;
+    }
+    const int tiles = (end - c0 + kThreads * kVectors * kVec - 1) / (kThreads * kVectors * kVec);
+    uint4 next[kVectors];
+#pragma unroll
+    for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, c0 + (u * kThreads + tid) * kVec, end, a.vocab);
+    float ref = -FLT_MAX;
+    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    for (int tile = 0; tile < tiles; ++tile) {
+        uint32_t w[kWords];
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) w[4 * u] = next[u].x, w[4 * u + 1] = next[u].y, w[4 * u + 2] = next[u].z, w[4 * u + 3] = next[u].w;
+        const int vec0 = tile * kThreads * kVectors + tid;
+        if (tile + 1 < tiles) {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u)
+                next[u] = load_vector<T, ALIGNED>(row, c0 + (vec0 + (kVectors + u) * kThreads) * kVec, end, a.vocab);
+        }
+        // ---- the tile's maximum; masked tokens are -inf from here on
+        const auto maximum = [&] {
+            uint32_t m = w[0];
+#pragma unroll
+            for (int i = 1; i < kWords; ++i) m = max_words<T>(m, w[i]);
+            const float2 f = pair_of<T>(m);
+            return fmaxf(f.x, f.y);
+        };
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = without_nan<T>(w[i]);
+        float top = maximum();
+        if (top == INFINITY) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    if (w[i] == 0x7f800000u) w[i] = Type<T>::kMasked;
+                } else {
+                    const float2 f = pair_of<T>(w[i]);
+                    if (f.x == INFINITY) w[i] = (w[i] & 0xffff0000u) | (Type<T>::kMasked & 0xffffu);
+                    if (f.y == INFINITY) w[i] = (w[i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
+                }
+            }
+            top = maximum();
+        }
+        // ---- sum of exp(x - ref)
+        if (top - ref > kGrow) {
+            const float f = exp2_approx((ref - top) * kLog2e);
+            ref = top;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sum[i] = make_float2(sum[i].x * f, sum[i].y * f);
+        }
+        const float2 minus = {-ref, -ref}, scale = {kLog2e, kLog2e};
+#pragma unroll
+        for (int i = 0; i < kWords; i += sizeof(T) == 4 ? 2 : 1) {
+            float2 x;
+            if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+            else x = pair_of<T>(w[i]);
+            const float2 y = mul2(add2(x, minus), scale);
+            sum[sizeof(T) == 4 ? i / 2 & 1 : i & 1] = add2(sum[sizeof(T) == 4 ? i / 2 & 1 : i & 1], make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+        }
+        // ---- candidates
+        float bound;
+        bool pass;
+        if (tile == 0) {
+            // maxima over 2 or 4 neighbouring threads: at least twice k of them
+            float part = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            const int by = k <= 32 ? 4 : 2, parts = kThreads / by;
+            if (by == 4) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 2));
+            if (tid % by == 0) sh.part_max[tid / by] = part;
+            __syncthreads();
+            if (tid < parts) {
+                const float mine = sh.part_max[tid];
+                int rank = 0;
+                for (int i = 0; i < parts; ++i) {
+                    const float other = sh.part_max[i];
+                    rank += other > mine || (other == mine && i < tid);
+                }
+                if (rank == k - 1) sh.bound = mine;
+            }
+            __syncthreads();
+            bound = sh.bound;
+            pass = top >= bound && top > -INFINITY;
+        } else {
+            bound = sh.bound;
+            pass = top > bound;      // (an equal logit of a later token loses against those that made the bound)
+        }
+        bool lost = false;
+        if (pass) {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const float x = element<T>(w, u * kVec + e);
+                    if (x > bound || (tile == 0 && x == bound && x > -INFINITY)) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(c0 + (vec0 + u * kThreads) * kVec + e));
+                        else lost = true;
+                    }
+                }
+        }
+        if (__syncthreads_or(lost)) select_exactly<T>(sh, w, vec0, c0, c0 + tile * kThreads * kVectors * kVec, k);
+    }
+
+    // ---- the chunk's sum, over the largest reference
+    const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    float most = ref;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) sh.warp_ref[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) most = fmaxf(most, sh.warp_ref[i]);
+    double total = all * exp2_approx((ref - most) * kLog2e);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) sh.warp_sum[warp] = total;
+    if (sh.count > kThreads) {      // more than a thread each: down to the k largest
+        uint32_t none[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) none[i] = Type<T>::kMasked;
+        __syncthreads();
+        select_exactly<T>(sh, none, 0, 0, INT_MAX, k);
+    } else {
+        __syncthreads();
+    }
+    const int64_t part = static_cast<int64_t>(row_number) * p.chunks + number;
+    if (tid == 0) {
+        double s = 0;
+        for (int i = 0; i < kWarps; ++i) s += sh.warp_sum[i];
+        p.partials[part] = {s, most, 0.f};
+    }
+    const int n = sh.count;
+    Key* out = p.lists + part * k;
+    if (tid < n) {
+        const Key mine = sh.list[tid];
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += sh.list[i] > mine;
+        if (rank < k) out[rank] = mine;
+    }
+    if (tid >= n && tid < k) out[tid] = 0;
+}
+
+// All lists of a group, by the CTA that finished its last chunk.
+__device__ __forceinline__ void merge(Shared& sh, const Params& p, int g) {
+    const wuda_beam_select_args& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k, chunks = p.chunks;
+    const int lists = a.width * chunks, entries = lists * k;
+    for (int w = warp; w < a.width; w += kWarps) {
+        const int row = g * a.width + w;
+        const float score = a.scores[row];
+        const bool dead = !(fabsf(score) < INFINITY), done = !dead && a.finished && a.finished[row];
+        double lse = 0;
+        if (!dead && !done) {
+            const Partial* parts = p.partials + static_cast<int64_t>(row) * chunks;
+            float most = -FLT_MAX;
+            for (int i = lane; i < chunks; i += 32) most = fmaxf(most, __ldcg(&parts[i].ref));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            double total = 0;
+            for (int i = lane; i < chunks; i += 32) total += __ldcg(&parts[i].sum) * exp(static_cast<double>(__ldcg(&parts[i].ref)) - most);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+            lse = most + log(total);
+        }
+        if (lane == 0) sh.lse[w] = lse, sh.score[w] = score, sh.kind[w] = dead ? 2 : done;
+    }
+    if (tid == 0) sh.survivors = sh.there = 0, sh.least = -INFINITY;
+    __syncthreads();
+    const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
     for (int e = tid; e < entries; e += kThreads) {
-        const int row = g * a.width + e / a.k;
-        const double score = a.scores[row];
+        const int list = e / k, w = list / chunks;
+        Key key = 0;
         double v = -INFINITY;
-        if (fabs(score) < INFINITY) {
-            if (a.finished && a.finished[row]) {
-                if (e % a.k == 0) v = score;
-            } else if (const unsigned long long key = p.lists[static_cast<int64_t>(row) * a.k + e % a.k]) {
-                v = (score + unordered(static_cast<uint32_t>(key >> 32))) - p.lse[row];
+        if (sh.kind[w] == 0) {
+            key = __ldcg(keys + e);
+            if (key) v = (sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w];
+        } else if (sh.kind[w] == 1 && e == w * chunks * k) {
+            v = sh.score[w];
+            key = key_of(0.f, static_cast<uint32_t>(a.eos_token));
+        }
+        sh.list[e] = key;
+        sh.value[e] = v;
+    }
+    __syncthreads();
+    // the k-th largest value among the first `deep` of every list: nothing below it is among the k best
+    const int deep = (k + lists - 1) / lists, pool = lists * deep;
+    for (int i = tid; i < pool; i += kThreads) {
+        const double mine = sh.value[i / deep * k + i % deep];
+        int rank = 0;
+        for (int l = 0, at = 0; l < lists; ++l)
+            for (int d = 0; d < deep; ++d, ++at) {
+                const double other = sh.value[l * k + d];
+                rank += other > mine || (other == mine && at < i);
+            }
+        if (rank == k - 1) sh.least = mine;
+    }
+    __syncthreads();
+    const double least = sh.least;
+    for (int e = tid; e < entries; e += kThreads)
+        if (sh.list[e] && sh.value[e] >= least) sh.passed[atomicAdd(&sh.survivors, 1)] = static_cast<uint16_t>(e);
+    __syncthreads();
+    const int n = sh.survivors;
+    for (int i = tid; i < n; i += kThreads) {
+        const int e = sh.passed[i], w = e / (k * chunks);
+        const double mine = sh.value[e];
+        const Key key = sh.list[e];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) {
+            const int o = sh.passed[j];
+            const double other = sh.value[o];
+            if (other > mine) ++rank;
+            else if (other == mine && o != e) {
+                const int ow = o / (k * chunks);
+                rank += ow != w ? ow < w : sh.list[o] > key;      // lower beam; within a beam larger logit, lower token
             }
         }
-        value[e] = v;
+        if (rank >= k) continue;
+        atomicAdd(&sh.there, 1);
+        const int64_t at = static_cast<int64_t>(g) * k + rank;
+        const int token = static_cast<int>(token_of(key));
+        a.scores_out[at] = static_cast<float>(mine);
+        a.parents_out[at] = w;
+        a.tokens_out[at] = token;
+        a.finished_out[at] = sh.kind[w] == 1 || token == a.eos_token;
     }
     __syncthreads();
-    for (int e = 0; e < entries; ++e) there += value[e] > -INFINITY;
-    for (int e = tid; e < entries; e += kThreads) {
-        const double v = value[e];
-        if (v == -INFINITY) continue;
-        int rank = 0;
-        for (int o = 0; o < entries; ++o) rank += value[o] > v || (value[o] == v && o < e);
-        if (rank >= a.k) continue;
-        const int beam = e / a.k, row = g * a.width + beam;
-        const bool done = a.finished && a.finished[row];
-        const int token = done ? a.eos_token : static_cast<int>(~static_cast<uint32_t>(p.lists[static_cast<int64_t>(row) * a.k + e % a.k]));
-        const int64_t at = static_cast<int64_t>(g) * a.k + rank;
-        a.scores_out[at] = static_cast<float>(v);
-        a.parents_out[at] = beam;
-        a.tokens_out[at] = token;
-        a.finished_out[at] = done || token == a.eos_token;
-    }
-    for (int j = there + tid; j < a.k; j += kThreads) {
-        const int64_t at = static_cast<int64_t>(g) * a.k + j;
+    for (int j = sh.there + tid; j < k; j += kThreads) {
+        const int64_t at = static_cast<int64_t>(g) * k + j;
         a.scores_out[at] = -INFINITY;
         a.parents_out[at] = a.tokens_out[at] = -1;
         a.finished_out[at] = 0;
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ Params p) {
+    __shared__ Shared sh;
+    const wuda_beam_select_args& a = p.a;
+    pdl_launch_dependents();
+    pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
+    const int number = blockIdx.x % p.chunks, row = blockIdx.x / p.chunks, g = row / a.width;
+    const float score = a.scores[row];
+    if (fabsf(score) < INFINITY && !(a.finished && a.finished[row])) {
+        const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
+        if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) chunk<T, true>(sh, p, x, row, number);
+        else chunk<T, false>(sh, p, x, row, number);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned all = a.width * p.chunks - 1;
+        sh.last = atomicInc(reinterpret_cast<unsigned*>(a.counters + g), all) == all;      // (wraps back to zero)
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    merge(sh, p, g);
+}
+
+// Chunks of a row: enough CTAs for the device and whole rounds of loads for each, and lists that the merge can hold.
+void cut(int groups, int width, int vocab, int k, int type, int* chunks, int* chunk_vectors) {
+    const int vec = type == 2 ? 4 : 8, rows = groups * width;
+    const int blocks = (vocab + vec * kThreads - 1) / (vec * kThreads);      // rounds of one load per thread
+    int n = (kCtas + rows - 1) / rows;
+    n = std::min(std::min(n, blocks), std::min(kMostChunks, kList / (width * k)));
+    const int per = (blocks + n - 1) / n;
+    *chunks = (blocks + per - 1) / per;
+    *chunk_vectors = per * kThreads;
 }
 
 bool sizes_fit(int groups, int width, int vocab, int k, int type) {
@@ -151,7 +555,10 @@ bool sizes_fit(int groups, int width, int vocab, int k, int type) {
 extern "C" int64_t wuda_beam_select_workspace_bytes(int groups, int width, int vocab, int k, int logits_type) {
     using namespace wuda::beams;
     if (!sizes_fit(groups, width, vocab, k, logits_type)) return -1;
-    return static_cast<int64_t>(groups) * width * (k + 1) * 8;
+    if (groups == 0) return 0;
+    int chunks, vectors;
+    cut(groups, width, vocab, k, logits_type, &chunks, &vectors);
+    return static_cast<int64_t>(groups) * width * chunks * (k * sizeof(Key) + sizeof(Partial));
 }
 
 extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream) {
@@ -177,15 +584,13 @@ extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream)
                  static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
     DeviceInfo dev;
     if (const int st = current_device_info(&dev)) return st;
-    const int rows = a.groups * a.width;
     Params p;
     p.a = a;
-    p.lists = static_cast<unsigned long long*>(a.workspace);
-    p.lse = reinterpret_cast<double*>(p.lists + static_cast<int64_t>(rows) * a.k);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a.logits_type == 0) WUDA_CUDA(launch_pdl(beam_rows_kernel<__nv_bfloat16>, dim3(rows), dim3(kThreads), 0, s, p));
-    if (a.logits_type == 1) WUDA_CUDA(launch_pdl(beam_rows_kernel<__half>, dim3(rows), dim3(kThreads), 0, s, p));
-    if (a.logits_type == 2) WUDA_CUDA(launch_pdl(beam_rows_kernel<float>, dim3(rows), dim3(kThreads), 0, s, p));
-    WUDA_CUDA(launch_pdl(beam_merge_kernel, dim3(a.groups), dim3(kThreads), 0, s, p));
+    cut(a.groups, a.width, a.vocab, a.k, a.logits_type, &p.chunks, &p.chunk_vectors);
+    const int64_t parts = static_cast<int64_t>(a.groups) * a.width * p.chunks;
+    p.partials = static_cast<Partial*>(a.workspace);
+    p.lists = reinterpret_cast<Key*>(p.partials + parts);
+    void (*kernel)(Params) = a.logits_type == 0 ? beam_select_kernel<__nv_bfloat16> : a.logits_type == 1 ? beam_select_kernel<__half> : beam_select_kernel<float>;
+    WUDA_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }
