@@ -11,9 +11,9 @@
 // where a term would pass e^40: a rescaling is rare, and no term overflows).  Which element a thread gets depends on the element's number
 // alone, not on the row's alignment, so equal rows have equal sums.
 //
-// Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the first tile is a lower bound of the row's k-th
-// largest logit; only what passes it (a handful per tile) goes to a list in shared memory.  A tile that overflows the list (sorted rows,
-// rows of one value) ends in an exact selection over list and tile, which leaves the k largest and a new bound.
+// Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's k-th largest
+// logit, raised in front of the tiles 0, 1, 3, 7, ..; only what passes it (a handful per tile) goes to a list in shared memory.  No
+// barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
 // The CTA that completes a group's counter merges its lists: the k-th largest of the lists' first candidates bounds what can be among
 // the k best, and the few that pass are ranked by counting.
@@ -36,6 +36,8 @@ constexpr int kVectors = 4;                 // 16-byte loads per thread and tile
 constexpr int kMostK = 64, kMostWidth = 32, kMostGroups = 256;
 constexpr int kList = 2048;                 // candidates that a CTA holds, and that a group's chunks may have together
 constexpr int kMostChunks = 64;
+constexpr int kMostLists = 1024;            // of a group
+constexpr int kFront = kMostLists + kMostK; // the lists' first candidates, at least k of them
 constexpr int kCtas = 1184;                 // CTAs of a launch: eight per SM, taken as SMs come free
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
@@ -181,33 +183,36 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit typ
     else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
     else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-// element e of a tile's 16 words
-template <typename T>
-__device__ __forceinline__ float element(const uint32_t (&w)[4 * kVectors], int e) {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
-    else {
-        const float2 f = pair_of<T>(w[e / 2]);
-        return e & 1 ? f.y : f.x;
-    }
-}
-
 struct Shared {
-    Key list[kList];
+    alignas(16) Key list[kList];
     int count;                              // candidates pushed (those beyond kList are lost)
     float bound;                            // the k-th largest logit so far, or less
-    float part_max[128];                    // maxima of parts of a tile
+    alignas(16) float part_max[128];        // maxima of parts of the tiles
     int hits[2];
     float warp_ref[kWarps];
     double warp_sum[kWarps];
     bool last;
     // merging
-    double value[kList];
+    Key value[kList];
+    alignas(16) Key front[kFront];
     uint16_t passed[kList];
     double lse[kMostWidth], score[kMostWidth];
     int kind[kMostWidth];
-    double least;
+    Key least;
     int survivors, there;
 };
+
+// How many of n keys are larger, two at a time.
+__device__ __forceinline__ int larger_than(Key mine, const Key* keys, int n) {
+    int rank = 0, i = 0;
+#pragma unroll 4
+    for (; i + 1 < n; i += 2) {
+        const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(keys + i);
+        rank += (other.x > mine) + (other.y > mine);
+    }
+    if (i < n) rank += keys[i] > mine;
+    return rank;
+}
 
 __device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
     const int n = __reduce_add_sync(0xffffffffu, mine);
@@ -219,24 +224,16 @@ __device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
     return total;
 }
 
-// The k largest of the list's entries of tokens below `first_token` and the tile's elements, exactly: the largest K such that k keys are at
-// or above it, bit by bit.  They become the list.  All threads; ends behind a barrier.
-template <typename T>
-__device__ __noinline__ void select_exactly(Shared& sh, const uint32_t (&w)[4 * kVectors], int vec0, int c0, int tile_base, int k) {
-    constexpr int kVec = Type<T>::kVec;
+// The k largest of the list and of the tile's keys, exactly: the largest K such that k of them are at or above it, bit by bit.  They become
+// the list (all of them where they are fewer).  Returns K.  All threads; ends behind a barrier.
+template <int N>
+__device__ Key select_exactly(Shared& sh, const Key (&tile)[N], int k) {
     Key held[kList / kThreads];
     const int count = min(sh.count, kList);
 #pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) {
-        const int at = i * kThreads + threadIdx.x;
-        held[i] = at < count && token_of(sh.list[at]) < static_cast<uint32_t>(tile_base) ? sh.list[at] : 0;
-    }
+    for (int i = 0; i < kList / kThreads; ++i) held[i] = i * kThreads + threadIdx.x < count ? sh.list[i * kThreads + threadIdx.x] : 0;
     if (threadIdx.x == 0) sh.hits[0] = sh.hits[1] = 0;
     __syncthreads();
-    const auto tile_key = [&](int u, int e) -> Key {
-        const float x = element<T>(w, u * kVec + e);
-        return x > -INFINITY ? key_of(x, static_cast<uint32_t>(c0 + (vec0 + u * kThreads) * kVec + e)) : 0;
-    };
     Key least = 0;
     for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
         const Key want = least | (1ull << bit);
@@ -244,9 +241,7 @@ __device__ __noinline__ void select_exactly(Shared& sh, const uint32_t (&w)[4 * 
 #pragma unroll
         for (int i = 0; i < kList / kThreads; ++i) mine += held[i] >= want;
 #pragma unroll
-        for (int u = 0; u < kVectors; ++u)
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) mine += tile_key(u, e) >= want;
+        for (int i = 0; i < N; ++i) mine += tile[i] >= want;
         const int total = block_total(mine, sh.hits, turn);
         if (total >= k) least = want;
         if (total == k) break;
@@ -259,18 +254,48 @@ __device__ __noinline__ void select_exactly(Shared& sh, const uint32_t (&w)[4 * 
 #pragma unroll
     for (int i = 0; i < kList / kThreads; ++i) keep(held[i]);
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u)
+    for (int i = 0; i < N; ++i) keep(tile[i]);
+    __syncthreads();
+    return least;
+}
+__device__ __noinline__ void trim_list(Shared& sh, int k) {
+    const Key none[1] = {0};
+    select_exactly(sh, none, k);
+}
+
+// A chunk's k largest keys where the list overflowed (rows sorted upwards, rows of one value, rows masked but for their end): tile by tile with
+// exact selections, as far as a tile has a key above the k-th largest so far.
+template <typename T>
+__device__ __noinline__ void candidates_exactly(Shared& sh, const T* row, int c0, int end, int vocab, int k) {
+    constexpr int kVec = Type<T>::kVec;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    Key least = 0;
+    for (int at = c0; at < end; at += kThreads * kVec) {
+        const int first = at + threadIdx.x * kVec;
+        const uint4 v = load_vector<T, false>(row, first, end, vocab);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        Key keys[kVec];
+        bool above = false;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) keep(tile_key(u, e));
-    __syncthreads();
-    if (threadIdx.x == 0 && sh.count == k) sh.bound = unordered(static_cast<uint32_t>(least >> 32));
-    __syncthreads();
+        for (int e = 0; e < kVec; ++e) {
+            const float2 f = pair_of<T>(w[e * 4 / kVec]);
+            const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
+            keys[e] = fabsf(x) < INFINITY ? key_of(x, static_cast<uint32_t>(first + e)) : 0;
+            above = above || keys[e] > least;
+        }
+        if (__syncthreads_or(above)) {
+            const Key now = select_exactly(sh, keys, k);
+            if (sh.count == k) least = now;
+            __syncthreads();
+        }
+    }
 }
 
 // A chunk of a row: its partial sum, and its k largest keys in descending order.
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row, int row_number, int number) {
-    constexpr int kVec = Type<T>::kVec, kWords = 4 * kVectors;
+    constexpr int kVec = Type<T>::kVec;
     const wuda_beam_select_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
     const int c0 = number * p.chunk_vectors * kVec, end = min(a.vocab, c0 + p.chunk_vectors * kVec);
@@ -282,41 +307,48 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
     uint4 next[kVectors];
 #pragma unroll
     for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, c0 + (u * kThreads + tid) * kVec, end, a.vocab);
-    float ref = -FLT_MAX;
+    float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 1, 3, 7, ..
     for (int tile = 0; tile < tiles; ++tile) {
-        uint32_t w[kWords];
+        uint32_t w[kVectors][4];
 #pragma unroll
-        for (int u = 0; u < kVectors; ++u) w[4 * u] = next[u].x, w[4 * u + 1] = next[u].y, w[4 * u + 2] = next[u].z, w[4 * u + 3] = next[u].w;
-        const int vec0 = tile * kThreads * kVectors + tid;
+        for (int u = 0; u < kVectors; ++u) {
+            w[u][0] = without_nan<T>(next[u].x), w[u][1] = without_nan<T>(next[u].y);
+            w[u][2] = without_nan<T>(next[u].z), w[u][3] = without_nan<T>(next[u].w);
+        }
+        const int e0 = c0 + (tile * kThreads * kVectors + tid) * kVec;      // first element of the thread's first vector
         if (tile + 1 < tiles) {
 #pragma unroll
             for (int u = 0; u < kVectors; ++u)
-                next[u] = load_vector<T, ALIGNED>(row, c0 + (vec0 + (kVectors + u) * kThreads) * kVec, end, a.vocab);
+                next[u] = load_vector<T, ALIGNED>(row, e0 + (kVectors + u) * kThreads * kVec, end, a.vocab);
         }
-        // ---- the tile's maximum; masked tokens are -inf from here on
-        const auto maximum = [&] {
-            uint32_t m = w[0];
+        // ---- the vectors' maxima; masked tokens are -inf from here on
+        float high[kVectors], top;
+        const auto maxima = [&] {
+            top = -INFINITY;
 #pragma unroll
-            for (int i = 1; i < kWords; ++i) m = max_words<T>(m, w[i]);
-            const float2 f = pair_of<T>(m);
-            return fmaxf(f.x, f.y);
+            for (int u = 0; u < kVectors; ++u) {
+                const float2 f = pair_of<T>(max_words<T>(max_words<T>(w[u][0], w[u][1]), max_words<T>(w[u][2], w[u][3])));
+                high[u] = fmaxf(f.x, f.y);
+                top = fmaxf(top, high[u]);
+            }
         };
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = without_nan<T>(w[i]);
-        float top = maximum();
+        maxima();
         if (top == INFINITY) {
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    if (w[i] == 0x7f800000u) w[i] = Type<T>::kMasked;
-                } else {
-                    const float2 f = pair_of<T>(w[i]);
-                    if (f.x == INFINITY) w[i] = (w[i] & 0xffff0000u) | (Type<T>::kMasked & 0xffffu);
-                    if (f.y == INFINITY) w[i] = (w[i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
+            for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = pair_of<T>(w[u][i]);
+                    if constexpr (sizeof(T) == 4) {
+                        if (f.x == INFINITY) w[u][i] = Type<T>::kMasked;
+                    } else {
+                        if (f.x == INFINITY) w[u][i] = (w[u][i] & 0xffff0000u) | (Type<T>::kMasked & 0xffffu);
+                        if (f.y == INFINITY) w[u][i] = (w[u][i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
+                    }
                 }
-            }
-            top = maximum();
+            maxima();
         }
         // ---- sum of exp(x - ref)
         if (top - ref > kGrow) {
@@ -327,54 +359,57 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
         }
         const float2 minus = {-ref, -ref}, scale = {kLog2e, kLog2e};
 #pragma unroll
-        for (int i = 0; i < kWords; i += sizeof(T) == 4 ? 2 : 1) {
-            float2 x;
-            if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
-            else x = pair_of<T>(w[i]);
-            const float2 y = mul2(add2(x, minus), scale);
-            sum[sizeof(T) == 4 ? i / 2 & 1 : i & 1] = add2(sum[sizeof(T) == 4 ? i / 2 & 1 : i & 1], make_float2(exp2_approx(y.x), exp2_approx(y.y)));
-        }
+        for (int u = 0; u < kVectors; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; i += sizeof(T) == 4 ? 2 : 1) {
+                float2 x;
+                if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[u][i]), __uint_as_float(w[u][i + 1]));
+                else x = pair_of<T>(w[u][i]);
+                const float2 y = mul2(add2(x, minus), scale);
+                const int to = sizeof(T) == 4 ? i / 2 : i & 1;
+                sum[to] = add2(sum[to], make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+            }
         // ---- candidates
-        float bound;
-        bool pass;
-        if (tile == 0) {
-            // maxima over 2 or 4 neighbouring threads: at least twice k of them
-            float part = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        so_far = fmaxf(so_far, top);
+        bool with_equal = false;      // a logit equal to the bound is a candidate where the bound is this tile's
+        if (tile == refresh) {
+            refresh = 2 * refresh + 1;
+            // maxima over 2 or 4 neighbouring threads and all tiles so far: at least twice k of them
+            float part = fmaxf(so_far, __shfl_xor_sync(0xffffffffu, so_far, 1));
             const int by = k <= 32 ? 4 : 2, parts = kThreads / by;
             if (by == 4) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 2));
             if (tid % by == 0) sh.part_max[tid / by] = part;
             __syncthreads();
             if (tid < parts) {
                 const float mine = sh.part_max[tid];
-                int rank = 0;
-                for (int i = 0; i < parts; ++i) {
-                    const float other = sh.part_max[i];
-                    rank += other > mine || (other == mine && i < tid);
+                int larger = 0, not_smaller = 0;
+#pragma unroll 4
+                for (int i = 0; i < parts; i += 4) {
+                    const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[i]);
+                    larger += (other.x > mine) + (other.y > mine) + (other.z > mine) + (other.w > mine);
+                    not_smaller += (other.x >= mine) + (other.y >= mine) + (other.z >= mine) + (other.w >= mine);
                 }
-                if (rank == k - 1) sh.bound = mine;
+                if (larger < k && k <= not_smaller) sh.bound = mine;      // (equal ones write the same)
             }
             __syncthreads();
+            with_equal = sh.bound > bound;
             bound = sh.bound;
-            pass = top >= bound && top > -INFINITY;
-        } else {
-            bound = sh.bound;
-            pass = top > bound;      // (an equal logit of a later token loses against those that made the bound)
         }
-        bool lost = false;
-        if (pass) {
+        if (with_equal ? top >= bound : top > bound) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u)
+            for (int u = 0; u < kVectors; ++u) {
+                if (high[u] < bound) continue;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    const float x = element<T>(w, u * kVec + e);
-                    if (x > bound || (tile == 0 && x == bound && x > -INFINITY)) {
+                    const float2 f = pair_of<T>(w[u][e * 4 / kVec]);
+                    const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
+                    if (x > bound || (with_equal && x == bound)) {
                         const int at = atomicAdd(&sh.count, 1);
-                        if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(c0 + (vec0 + u * kThreads) * kVec + e));
-                        else lost = true;
+                        if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(e0 + u * kThreads * kVec + e));
                     }
                 }
+            }
         }
-        if (__syncthreads_or(lost)) select_exactly<T>(sh, w, vec0, c0, c0 + tile * kThreads * kVectors * kVec, k);
     }
 
     // ---- the chunk's sum, over the largest reference
@@ -390,12 +425,11 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) sh.warp_sum[warp] = total;
-    if (sh.count > kThreads) {      // more than a thread each: down to the k largest
-        uint32_t none[kWords];
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) none[i] = Type<T>::kMasked;
+    if (sh.count > kThreads) {
+        const bool lost = sh.count > kList;
         __syncthreads();
-        select_exactly<T>(sh, none, 0, 0, INT_MAX, k);
+        if (lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
+        else trim_list(sh, k);      // more than a thread each: down to the k largest
     } else {
         __syncthreads();
     }
@@ -409,18 +443,29 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
     Key* out = p.lists + part * k;
     if (tid < n) {
         const Key mine = sh.list[tid];
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += sh.list[i] > mine;
+        const int rank = larger_than(mine, sh.list, n);
         if (rank < k) out[rank] = mine;
     }
     if (tid >= n && tid < k) out[tid] = 0;
 }
 
+// a word that grows with the value; 0 is below every number
+__device__ __forceinline__ Key ordered(double x) {
+    const long long b = __double_as_longlong(x);
+    return static_cast<Key>(b) ^ (static_cast<Key>(b >> 63) | (1ull << 63));
+}
+__device__ __forceinline__ double unordered(Key u) { return __longlong_as_double(u & (1ull << 63) ? u ^ (1ull << 63) : ~u); }
+
 // All lists of a group, by the CTA that finished its last chunk.
-__device__ __forceinline__ void merge(Shared& sh, const Params& p, int g) {
+__device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     const wuda_beam_select_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k, chunks = p.chunks;
-    const int lists = a.width * chunks, entries = lists * k;
+    const int per_beam = chunks * k, lists = a.width * chunks, entries = lists * k;
+    // the lists' keys are on their way while the beams' sums are added
+    const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
+    Key mine[kList / kThreads];
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) mine[i] = i * kThreads + tid < entries ? __ldcg(keys + i * kThreads + tid) : 0;
     for (int w = warp; w < a.width; w += kWarps) {
         const int row = g * a.width + w;
         const float score = a.scores[row];
@@ -428,73 +473,103 @@ __device__ __forceinline__ void merge(Shared& sh, const Params& p, int g) {
         double lse = 0;
         if (!dead && !done) {
             const Partial* parts = p.partials + static_cast<int64_t>(row) * chunks;
-            float most = -FLT_MAX;
-            for (int i = lane; i < chunks; i += 32) most = fmaxf(most, __ldcg(&parts[i].ref));
+            float ref[kMostChunks / 32], most = -FLT_MAX;
+            double sum[kMostChunks / 32], total = 0;
+#pragma unroll
+            for (int i = 0; i < kMostChunks / 32; ++i) {
+                const int at = i * 32 + lane;
+                ref[i] = at < chunks ? __ldcg(&parts[at].ref) : -FLT_MAX;
+                sum[i] = at < chunks ? __ldcg(&parts[at].sum) : 0;
+                most = fmaxf(most, ref[i]);
+            }
 #pragma unroll
             for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            double total = 0;
-            for (int i = lane; i < chunks; i += 32) total += __ldcg(&parts[i].sum) * exp(static_cast<double>(__ldcg(&parts[i].ref)) - most);
+#pragma unroll
+            for (int i = 0; i < kMostChunks / 32; ++i) total += sum[i] * exp(static_cast<double>(ref[i]) - most);
 #pragma unroll
             for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
             lse = most + log(total);
         }
         if (lane == 0) sh.lse[w] = lse, sh.score[w] = score, sh.kind[w] = dead ? 2 : done;
     }
-    if (tid == 0) sh.survivors = sh.there = 0, sh.least = -INFINITY;
+    if (tid == 0) sh.survivors = sh.there = 0, sh.least = 0;
     __syncthreads();
-    const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
-    for (int e = tid; e < entries; e += kThreads) {
-        const int list = e / k, w = list / chunks;
-        Key key = 0;
-        double v = -INFINITY;
-        if (sh.kind[w] == 0) {
-            key = __ldcg(keys + e);
-            if (key) v = (sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w];
-        } else if (sh.kind[w] == 1 && e == w * chunks * k) {
-            v = sh.score[w];
-            key = key_of(0.f, static_cast<uint32_t>(a.eos_token));
-        }
-        sh.list[e] = key;
-        sh.value[e] = v;
-    }
-    __syncthreads();
-    // the k-th largest value among the first `deep` of every list: nothing below it is among the k best
+    // values as ordered words; the first `deep` of every list also side by side
     const int deep = (k + lists - 1) / lists, pool = lists * deep;
-    for (int i = tid; i < pool; i += kThreads) {
-        const double mine = sh.value[i / deep * k + i % deep];
-        int rank = 0;
-        for (int l = 0, at = 0; l < lists; ++l)
-            for (int d = 0; d < deep; ++d, ++at) {
-                const double other = sh.value[l * k + d];
-                rank += other > mine || (other == mine && at < i);
-            }
-        if (rank == k - 1) sh.least = mine;
+#pragma unroll
+    for (int i = 0; i < kList / kThreads; ++i) {
+        const int e = i * kThreads + tid;
+        if (e >= entries) break;
+        const int list = e / k, w = list / chunks;
+        Key v = 0;
+        if (sh.kind[w] == 0) {
+            if (mine[i]) v = ordered((sh.score[w] + unordered(static_cast<uint32_t>(mine[i] >> 32))) - sh.lse[w]);
+        } else if (sh.kind[w] == 1 && e == w * per_beam) {
+            v = ordered(sh.score[w]);
+            mine[i] = key_of(0.f, static_cast<uint32_t>(a.eos_token));
+        }
+        sh.list[e] = mine[i];
+        sh.value[e] = v;
+        if (e - list * k < deep) sh.front[list * deep + e - list * k] = v;
     }
     __syncthreads();
-    const double least = sh.least;
+    // the k-th largest of the front: nothing below it is among the k best
+    for (int i = tid; i < pool; i += kThreads) {
+        const Key v = sh.front[i];
+        int larger = 0, not_smaller = 0, j = 0;
+#pragma unroll 4
+        for (; j + 1 < pool; j += 2) {
+            const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.front[j]);
+            larger += (other.x > v) + (other.y > v);
+            not_smaller += (other.x >= v) + (other.y >= v);
+        }
+        if (j < pool) larger += sh.front[j] > v, not_smaller += sh.front[j] >= v;
+        if (larger < k && k <= not_smaller) sh.least = v;
+    }
+    __syncthreads();
+    const Key least = max(sh.least, 1ull);
+    // (the front's places are free now: the values that pass, side by side)
     for (int e = tid; e < entries; e += kThreads)
-        if (sh.list[e] && sh.value[e] >= least) sh.passed[atomicAdd(&sh.survivors, 1)] = static_cast<uint16_t>(e);
+        if (sh.value[e] >= least) sh.passed[atomicAdd(&sh.survivors, 1)] = static_cast<uint16_t>(e);
     __syncthreads();
     const int n = sh.survivors;
+    const bool few = n <= kFront;
+    if (few)
+        for (int i = tid; i < n; i += kThreads) sh.front[i] = sh.value[sh.passed[i]];
+    __syncthreads();
     for (int i = tid; i < n; i += kThreads) {
-        const int e = sh.passed[i], w = e / (k * chunks);
-        const double mine = sh.value[e];
-        const Key key = sh.list[e];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) {
-            const int o = sh.passed[j];
-            const double other = sh.value[o];
-            if (other > mine) ++rank;
-            else if (other == mine && o != e) {
-                const int ow = o / (k * chunks);
-                rank += ow != w ? ow < w : sh.list[o] > key;      // lower beam; within a beam larger logit, lower token
+        const int e = sh.passed[i], w = e / per_beam;
+        const Key v = sh.value[e];
+        int rank = 0, equal = 0;
+        if (few) {
+            int j = 0;
+#pragma unroll 4
+            for (; j + 1 < n; j += 2) {
+                const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.front[j]);
+                rank += (other.x > v) + (other.y > v);
+                equal += (other.x == v) + (other.y == v);
+            }
+            if (j < n) rank += sh.front[j] > v, equal += sh.front[j] == v;
+        } else {
+            for (int j = 0; j < n; ++j) {
+                const Key other = sh.value[sh.passed[j]];
+                rank += other > v;
+                equal += other == v;
             }
         }
         if (rank >= k) continue;
+        if (equal > 1) {      // lower beam; within a beam larger logit, lower token
+            const Key key = sh.list[e];
+            for (int j = 0; j < n; ++j) {
+                const int o = sh.passed[j], ow = o / per_beam;
+                if (sh.value[o] == v && o != e) rank += ow != w ? ow < w : sh.list[o] > key;
+            }
+            if (rank >= k) continue;
+        }
         atomicAdd(&sh.there, 1);
         const int64_t at = static_cast<int64_t>(g) * k + rank;
-        const int token = static_cast<int>(token_of(key));
-        a.scores_out[at] = static_cast<float>(mine);
+        const int token = static_cast<int>(token_of(sh.list[e]));
+        a.scores_out[at] = static_cast<float>(unordered(v));
         a.parents_out[at] = w;
         a.tokens_out[at] = token;
         a.finished_out[at] = sh.kind[w] == 1 || token == a.eos_token;
@@ -509,7 +584,7 @@ __device__ __forceinline__ void merge(Shared& sh, const Params& p, int g) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 3) beam_select_kernel(const __grid_constant__ Params p) {
     __shared__ Shared sh;
     const wuda_beam_select_args& a = p.a;
     pdl_launch_dependents();
@@ -538,7 +613,7 @@ void cut(int groups, int width, int vocab, int k, int type, int* chunks, int* ch
     const int vec = type == 2 ? 4 : 8, rows = groups * width;
     const int blocks = (vocab + vec * kThreads - 1) / (vec * kThreads);      // rounds of one load per thread
     int n = (kCtas + rows - 1) / rows;
-    n = std::min(std::min(n, blocks), std::min(kMostChunks, kList / (width * k)));
+    n = std::min(std::min(n, blocks), std::min(std::min(kMostChunks, kMostLists / width), kList / (width * k)));
     const int per = (blocks + n - 1) / n;
     *chunks = (blocks + per - 1) / per;
     *chunk_vectors = per * kThreads;
