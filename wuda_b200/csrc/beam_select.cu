@@ -12,8 +12,8 @@
 // alone, not on the row's alignment, so equal rows have equal sums.
 //
 // Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's k-th largest
-// logit, raised in front of the tiles 0, 1, 3, 7, ..; only what passes it (a handful per tile) goes to a list in shared memory.  No
-// barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
+// logit, raised in front of the tiles 0, 3, 15, ..; a vector of loads that passes it (a handful per tile) is noted and looked at in the
+// end, with the last bound.  No barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
 // The CTA that completes a group's counter merges its lists: the k-th largest of the lists' first candidates bounds what can be among
 // the k best, and the few that pass are ranked by counting.
@@ -185,7 +185,7 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit typ
 }
 struct Shared {
     alignas(16) Key list[kList];
-    int count;                              // candidates pushed (those beyond kList are lost)
+    int count, vectors;                     // candidates, and vectors that may hold some (those beyond kList are lost)
     float bound;                            // the k-th largest logit so far, or less
     alignas(16) float part_max[128];        // maxima of parts of the tiles
     int hits[2];
@@ -193,7 +193,10 @@ struct Shared {
     double warp_sum[kWarps];
     bool last;
     // merging
-    Key value[kList];
+    union {
+        Key value[kList];
+        int vector[kList];                  // (of a chunk: vectors with a logit beyond the bound of their tile)
+    };
     alignas(16) Key front[kFront];
     uint16_t passed[kList];
     double lse[kMostWidth], score[kMostWidth];
@@ -300,16 +303,18 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
     const int c0 = number * p.chunk_vectors * kVec, end = min(a.vocab, c0 + p.chunk_vectors * kVec);
     if (tid == 0) {
-        sh.count = 0;
+        sh.count = sh.vectors = 0;
         sh.bound = -INFINITY;
     }
+    const bool few = k <= 32;
+    const int by = few ? 4 : 2;
     const int tiles = (end - c0 + kThreads * kVectors * kVec - 1) / (kThreads * kVectors * kVec);
     uint4 next[kVectors];
 #pragma unroll
     for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, c0 + (u * kThreads + tid) * kVec, end, a.vocab);
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 1, 3, 7, ..
+    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, ..
     for (int tile = 0; tile < tiles; ++tile) {
         uint32_t w[kVectors][4];
 #pragma unroll
@@ -373,44 +378,63 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
         so_far = fmaxf(so_far, top);
         bool with_equal = false;      // a logit equal to the bound is a candidate where the bound is this tile's
         if (tile == refresh) {
-            refresh = 2 * refresh + 1;
-            // maxima over 2 or 4 neighbouring threads and all tiles so far: at least twice k of them
+            refresh = 4 * refresh + 3;
+            // maxima over 2 or 4 neighbouring threads and all tiles so far, at least twice k of them: 8 warps look for the k-th largest
             float part = fmaxf(so_far, __shfl_xor_sync(0xffffffffu, so_far, 1));
-            const int by = k <= 32 ? 4 : 2, parts = kThreads / by;
-            if (by == 4) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 2));
+            if (few) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 2));
             if (tid % by == 0) sh.part_max[tid / by] = part;
             __syncthreads();
-            if (tid < parts) {
-                const float mine = sh.part_max[tid];
-                int larger = 0, not_smaller = 0;
+            int larger = 0, not_smaller = 0;      // than the thread's own part, among a quarter or half of them
 #pragma unroll 4
-                for (int i = 0; i < parts; i += 4) {
-                    const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[i]);
-                    larger += (other.x > mine) + (other.y > mine) + (other.z > mine) + (other.w > mine);
-                    not_smaller += (other.x >= mine) + (other.y >= mine) + (other.z >= mine) + (other.w >= mine);
-                }
-                if (larger < k && k <= not_smaller) sh.bound = mine;      // (equal ones write the same)
+            for (int i = 0; i < kThreads / 16; i += 4) {
+                const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[few ? tid % 4 * 4 + i * 4 : tid % 2 * 4 + i * 2]);
+                larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
+                not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
             }
+            if (!few) {
+#pragma unroll 4
+                for (int i = kThreads / 16; i < kThreads / 4; i += 4) {
+                    const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[tid % 2 * 4 + i * 2]);
+                    larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
+                    not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
+                }
+            }
+            int both = larger | not_smaller << 16;
+            both += __shfl_xor_sync(0xffffffffu, both, 1);
+            if (few) both += __shfl_xor_sync(0xffffffffu, both, 2);
+            if ((both & 0xffff) < k && k <= both >> 16) sh.bound = part;      // (equal ones write the same)
             __syncthreads();
             with_equal = sh.bound > bound;
             bound = sh.bound;
         }
         if (with_equal ? top >= bound : top > bound) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-                if (high[u] < bound) continue;
+            for (int u = 0; u < kVectors; ++u)
+                if (with_equal ? high[u] >= bound : high[u] > bound) {
+                    const int at = atomicAdd(&sh.vectors, 1);
+                    if (at < kList) sh.vector[at] = (tile * kVectors + u) * kThreads + tid;
+                }
+        }
+    }
+
+    // ---- candidates: the elements of the noted vectors that pass the last bound
+    __syncthreads();
+    const int vectors = sh.vectors;
+    if (vectors <= kList)
+        for (int i = tid; i < vectors; i += kThreads) {
+            const int first = c0 + sh.vector[i] * kVec;
+            const uint4 v = load_vector<T, ALIGNED>(row, first, end, a.vocab);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    const float2 f = pair_of<T>(w[u][e * 4 / kVec]);
-                    const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
-                    if (x > bound || (with_equal && x == bound)) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(e0 + u * kThreads * kVec + e));
-                    }
+            for (int e = 0; e < kVec; ++e) {
+                const float2 f = pair_of<T>(w[e * 4 / kVec]);
+                const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
+                if (x >= bound && fabsf(x) < INFINITY) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(first + e));
                 }
             }
         }
-    }
 
     // ---- the chunk's sum, over the largest reference
     const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -425,8 +449,8 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) sh.warp_sum[warp] = total;
-    if (sh.count > kThreads) {
-        const bool lost = sh.count > kList;
+    if (sh.count > kThreads || vectors > kList) {
+        const bool lost = sh.count > kList || vectors > kList;
         __syncthreads();
         if (lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
         else trim_list(sh, k);      // more than a thread each: down to the k largest
