@@ -7,9 +7,10 @@
 // different beams are compared by value, in 64 bits.
 //
 // One launch.  A row of logits is cut into chunks, a CTA each, that are read once: 16 bytes per load, four loads per thread ahead of the
-// four that it works on.  Every thread keeps a reference r and the sum of exp(x - r) of its elements (r follows the maximum only
-// where a term would pass e^40: a rescaling is rare, and no term overflows).  Which element a thread gets depends on the element's number
-// alone, not on the row's alignment, so equal rows have equal sums.
+// four that it works on.  Every thread keeps a reference r and the sum of exp(x - r) of its elements; r follows the maximum only where a
+// term would pass e^40, so a rescaling is rare and no term overflows.  x - r is formed before the product with log2 e: the
+// largest logit counts exactly 1, a row of one token has log-probability 0, and logits of any magnitude will do.  Which element a
+// thread gets depends on the element's number alone, not on the row's alignment, so equal rows have equal sums.
 //
 // Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's k-th largest
 // logit, raised in front of the tiles 0, 3, 15, ..; a vector of loads that passes it (a handful per tile) is noted and looked at in the
@@ -30,15 +31,18 @@
 namespace wuda {
 namespace beams {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kVectors = 4;                 // 16-byte loads per thread and tile
 constexpr int kMostK = 64, kMostWidth = 32, kMostGroups = 256;
-constexpr int kList = 2048;                 // candidates that a CTA holds, and that a group's chunks may have together
+constexpr int kList = 1024;                 // candidates that a chunk's CTA holds, and vectors with candidates that it notes
+constexpr int kNotes = 384;                 // ... of which it keeps the contents
+constexpr int kEntries = 2048;              // candidates of all chunks of a group
 constexpr int kMostChunks = 64;
-constexpr int kMostLists = 1024;            // of a group
-constexpr int kFront = kMostLists + kMostK; // the lists' first candidates, at least k of them
-constexpr int kCtas = 1184;                 // CTAs of a launch: eight per SM, taken as SMs come free
+constexpr int kMostLists = 256;             // of a group
+constexpr int kFront = kMostLists + 4 * kMostK; // the lists' first candidates
+constexpr int kFew = 256;                   // values that are ranked side by side
+constexpr int kCtas = 1036;                 // CTAs of a launch: seven per SM, all at the same time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
 
@@ -184,25 +188,32 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit typ
     else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 struct Shared {
-    alignas(16) Key list[kList];
     int count, vectors;                     // candidates, and vectors that may hold some (those beyond kList are lost)
     float bound;                            // the k-th largest logit so far, or less
-    alignas(16) float part_max[128];        // maxima of parts of the tiles
     int hits[2];
     float warp_ref[kWarps];
     double warp_sum[kWarps];
     bool last;
-    // merging
     union {
-        Key value[kList];
-        int vector[kList];                  // (of a chunk: vectors with a logit beyond the bound of their tile)
+        struct {                            // a chunk
+            alignas(16) Key list[kList];
+            alignas(16) uint4 note[kNotes];
+            alignas(16) float part_max[kThreads];      // maxima of parts of the tiles
+            int vector[kList];                         // vectors with a logit beyond the bound of their tile
+        };
+        struct {                            // a group's lists
+            alignas(16) Key entry[kEntries];
+            alignas(16) Key value[kFew];
+            alignas(16) uint32_t front[kFront];        // values of the lists' first candidates, as ordered words
+            double sum[kMostLists], lse[kMostWidth], score[kMostWidth];
+            float ref[kMostLists];
+            int kind[kMostWidth];                      // 0 live, 1 finished, 2 dead
+            uint16_t passed[kEntries];
+            uint8_t beam[kFew];
+            uint32_t least;
+            int survivors, there;
+        };
     };
-    alignas(16) Key front[kFront];
-    uint16_t passed[kList];
-    double lse[kMostWidth], score[kMostWidth];
-    int kind[kMostWidth];
-    Key least;
-    int survivors, there;
 };
 
 // How many of n keys are larger, two at a time.
@@ -227,37 +238,44 @@ __device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
     return total;
 }
 
-// The k largest of the list and of the tile's keys, exactly: the largest K such that k of them are at or above it, bit by bit.  They become
-// the list (all of them where they are fewer).  Returns K.  All threads; ends behind a barrier.
+// The largest K such that at least `want` of the block's keys are at or above it, bit by bit from `bits` down; 0 where they are fewer.
+// each(f) calls f(key) for every key of the thread.  All threads; ends behind a barrier.
+template <typename Each>
+__device__ __forceinline__ Key kth_largest(int want, int bits, int* hits, const Each& each) {
+    if (threadIdx.x == 0) hits[0] = hits[1] = 0;
+    __syncthreads();
+    Key least = 0;
+    for (int bit = bits - 1, turn = 0; bit >= 0; --bit, turn ^= 1) {
+        const Key probe = least | (1ull << bit);
+        int mine = 0;
+        each([&](Key key) { mine += key >= probe; });
+        const int total = block_total(mine, hits, turn);
+        if (total >= want) least = probe;
+        if (total == want) break;
+    }
+    return least;
+}
+
+// The k largest of the list and of the tile's keys (unique ones, 0 none) become the list, or all of them where they are fewer.  Returns
+// the k-th.  All threads; ends behind a barrier.
 template <int N>
-__device__ Key select_exactly(Shared& sh, const Key (&tile)[N], int k) {
+__device__ __forceinline__ Key select_exactly(Shared& sh, const Key (&tile)[N], int k) {
     Key held[kList / kThreads];
     const int count = min(sh.count, kList);
 #pragma unroll
     for (int i = 0; i < kList / kThreads; ++i) held[i] = i * kThreads + threadIdx.x < count ? sh.list[i * kThreads + threadIdx.x] : 0;
-    if (threadIdx.x == 0) sh.hits[0] = sh.hits[1] = 0;
-    __syncthreads();
-    Key least = 0;
-    for (int bit = 63, turn = 0; bit >= 0; --bit, turn ^= 1) {
-        const Key want = least | (1ull << bit);
-        int mine = 0;
+    const auto each = [&](const auto& f) {
 #pragma unroll
-        for (int i = 0; i < kList / kThreads; ++i) mine += held[i] >= want;
+        for (int i = 0; i < kList / kThreads; ++i) f(held[i]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) mine += tile[i] >= want;
-        const int total = block_total(mine, sh.hits, turn);
-        if (total >= k) least = want;
-        if (total == k) break;
-    }
+        for (int i = 0; i < N; ++i) f(tile[i]);
+    };
+    const Key least = kth_largest(k, 64, sh.hits, each);
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    const auto keep = [&](Key key) {
+    each([&](Key key) {
         if (key != 0 && key >= least) sh.list[atomicAdd(&sh.count, 1)] = key;      // (k of them at most)
-    };
-#pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) keep(held[i]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) keep(tile[i]);
+    });
     __syncthreads();
     return least;
 }
@@ -295,6 +313,32 @@ __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row, int c0
     }
 }
 
+// The k-th largest of the maxima that the threads (k <= 32: pairs of them) have seen: k logits so far are at or above it.
+__device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
+    const int tid = threadIdx.x;
+    const bool pairs = k <= 32;
+    const float part = pairs ? fmaxf(so_far, __shfl_xor_sync(0xffffffffu, so_far, 1)) : so_far;
+    if (!pairs || tid % 2 == 0) sh.part_max[pairs ? tid / 2 : tid] = part;
+    __syncthreads();
+    int larger = 0, not_smaller = 0;      // than the thread's own part; each of a pair of threads counts half of them
+    const int n = pairs ? kThreads / 16 : kThreads / 4;
+    const float4* parts = reinterpret_cast<const float4*>(sh.part_max) + (pairs ? tid % 2 * n : 0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+        const float4 other = parts[i];
+        larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
+        not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
+    }
+    if (pairs) {
+        larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+        not_smaller += __shfl_xor_sync(0xffffffffu, not_smaller, 1);
+    }
+    if (larger < k && k <= not_smaller) sh.bound = part;      // (equal ones write the same)
+    __syncthreads();
+    *raised = sh.bound > bound;
+    return sh.bound;
+}
+
 // A chunk of a row: its partial sum, and its k largest keys in descending order.
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row, int row_number, int number) {
@@ -306,54 +350,54 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
         sh.count = sh.vectors = 0;
         sh.bound = -INFINITY;
     }
-    const bool few = k <= 32;
-    const int by = few ? 4 : 2;
-    const int tiles = (end - c0 + kThreads * kVectors * kVec - 1) / (kThreads * kVectors * kVec);
+    constexpr int kTile = kThreads * kVectors * kVec;
+    const int tiles = (end - c0 + kTile - 1) / kTile;
     uint4 next[kVectors];
+    const auto fetch = [&](int tile) {
+        const int at = c0 + tile * kTile + tid * kVec;
+        if (ALIGNED && c0 + (tile + 1) * kTile <= end) {
 #pragma unroll
-    for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, c0 + (u * kThreads + tid) * kVec, end, a.vocab);
+            for (int u = 0; u < kVectors; ++u) next[u] = load16(row + at + u * kThreads * kVec);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, at + u * kThreads * kVec, end, a.vocab);
+        }
+    };
+    if (a.finished && a.finished[row_number]) return;
+    fetch(0);      // on its way while the score is
+    if (!(fabsf(a.scores[row_number]) < INFINITY)) return;
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
     int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, ..
     for (int tile = 0; tile < tiles; ++tile) {
-        uint32_t w[kVectors][4];
+        uint32_t w[4 * kVectors];
 #pragma unroll
-        for (int u = 0; u < kVectors; ++u) {
-            w[u][0] = without_nan<T>(next[u].x), w[u][1] = without_nan<T>(next[u].y);
-            w[u][2] = without_nan<T>(next[u].z), w[u][3] = without_nan<T>(next[u].w);
+        for (int u = 0; u < kVectors; ++u) {      // masked tokens are -inf from here on
+            w[4 * u] = without_nan<T>(next[u].x), w[4 * u + 1] = without_nan<T>(next[u].y);
+            w[4 * u + 2] = without_nan<T>(next[u].z), w[4 * u + 3] = without_nan<T>(next[u].w);
         }
-        const int e0 = c0 + (tile * kThreads * kVectors + tid) * kVec;      // first element of the thread's first vector
-        if (tile + 1 < tiles) {
+        if (tile + 1 < tiles) fetch(tile + 1);
+        // ---- the maximum of some of the words
+        const auto maximum = [&](int from, int n) {
+            uint32_t m = w[from];
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u)
-                next[u] = load_vector<T, ALIGNED>(row, e0 + (kVectors + u) * kThreads * kVec, end, a.vocab);
-        }
-        // ---- the vectors' maxima; masked tokens are -inf from here on
-        float high[kVectors], top;
-        const auto maxima = [&] {
-            top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-                const float2 f = pair_of<T>(max_words<T>(max_words<T>(w[u][0], w[u][1]), max_words<T>(w[u][2], w[u][3])));
-                high[u] = fmaxf(f.x, f.y);
-                top = fmaxf(top, high[u]);
-            }
+            for (int i = 1; i < n; ++i) m = max_words<T>(m, w[from + i]);
+            const float2 f = pair_of<T>(m);
+            return fmaxf(f.x, f.y);
         };
-        maxima();
+        float top = maximum(0, 4 * kVectors);
         if (top == INFINITY) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = pair_of<T>(w[u][i]);
-                    if constexpr (sizeof(T) == 4) {
-                        if (f.x == INFINITY) w[u][i] = Type<T>::kMasked;
-                    } else {
-                        if (f.x == INFINITY) w[u][i] = (w[u][i] & 0xffff0000u) | (Type<T>::kMasked & 0xffffu);
-                        if (f.y == INFINITY) w[u][i] = (w[u][i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
-                    }
+            for (int i = 0; i < 4 * kVectors; ++i) {
+                const float2 f = pair_of<T>(w[i]);
+                if constexpr (sizeof(T) == 4) {
+                    if (f.x == INFINITY) w[i] = Type<T>::kMasked;
+                } else {
+                    if (f.x == INFINITY) w[i] = (w[i] & 0xffff0000u) | (Type<T>::kMasked & 0xffffu);
+                    if (f.y == INFINITY) w[i] = (w[i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
                 }
-            maxima();
+            }
+            top = maximum(0, 4 * kVectors);
         }
         // ---- sum of exp(x - ref)
         if (top - ref > kGrow) {
@@ -364,66 +408,43 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
         }
         const float2 minus = {-ref, -ref}, scale = {kLog2e, kLog2e};
 #pragma unroll
-        for (int u = 0; u < kVectors; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; i += sizeof(T) == 4 ? 2 : 1) {
-                float2 x;
-                if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[u][i]), __uint_as_float(w[u][i + 1]));
-                else x = pair_of<T>(w[u][i]);
-                const float2 y = mul2(add2(x, minus), scale);
-                const int to = sizeof(T) == 4 ? i / 2 : i & 1;
-                sum[to] = add2(sum[to], make_float2(exp2_approx(y.x), exp2_approx(y.y)));
-            }
+        for (int i = 0; i < 4 * kVectors; i += sizeof(T) == 4 ? 2 : 1) {
+            float2 x;
+            if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+            else x = pair_of<T>(w[i]);
+            const float2 y = mul2(add2(x, minus), scale);
+            const int to = sizeof(T) == 4 ? i / 2 & 1 : i & 1;
+            sum[to] = add2(sum[to], make_float2(exp2_approx(y.x), exp2_approx(y.y)));
+        }
         // ---- candidates
         so_far = fmaxf(so_far, top);
         bool with_equal = false;      // a logit equal to the bound is a candidate where the bound is this tile's
         if (tile == refresh) {
             refresh = 4 * refresh + 3;
-            // maxima over 2 or 4 neighbouring threads and all tiles so far, at least twice k of them: 8 warps look for the k-th largest
-            float part = fmaxf(so_far, __shfl_xor_sync(0xffffffffu, so_far, 1));
-            if (few) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, 2));
-            if (tid % by == 0) sh.part_max[tid / by] = part;
-            __syncthreads();
-            int larger = 0, not_smaller = 0;      // than the thread's own part, among a quarter or half of them
-#pragma unroll 4
-            for (int i = 0; i < kThreads / 16; i += 4) {
-                const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[few ? tid % 4 * 4 + i * 4 : tid % 2 * 4 + i * 2]);
-                larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
-                not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
-            }
-            if (!few) {
-#pragma unroll 4
-                for (int i = kThreads / 16; i < kThreads / 4; i += 4) {
-                    const float4 other = *reinterpret_cast<const float4*>(&sh.part_max[tid % 2 * 4 + i * 2]);
-                    larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
-                    not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
-                }
-            }
-            int both = larger | not_smaller << 16;
-            both += __shfl_xor_sync(0xffffffffu, both, 1);
-            if (few) both += __shfl_xor_sync(0xffffffffu, both, 2);
-            if ((both & 0xffff) < k && k <= both >> 16) sh.bound = part;      // (equal ones write the same)
-            __syncthreads();
-            with_equal = sh.bound > bound;
-            bound = sh.bound;
+            bound = raise_bound(sh, so_far, k, bound, &with_equal);
         }
         if (with_equal ? top >= bound : top > bound) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u)
-                if (with_equal ? high[u] >= bound : high[u] > bound) {
+            for (int u = 0; u < kVectors; ++u) {
+                const float high = maximum(4 * u, 4);
+                if (with_equal ? high >= bound : high > bound) {
                     const int at = atomicAdd(&sh.vectors, 1);
                     if (at < kList) sh.vector[at] = (tile * kVectors + u) * kThreads + tid;
+                    if (at < kNotes) sh.note[at] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                 }
+            }
         }
     }
 
     // ---- candidates: the elements of the noted vectors that pass the last bound
-    __syncthreads();
+    bool raised;
+    if (4 * (tiles - 1) + 3 != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
+    else __syncthreads();      // (it was raised with the last tile)
     const int vectors = sh.vectors;
     if (vectors <= kList)
         for (int i = tid; i < vectors; i += kThreads) {
             const int first = c0 + sh.vector[i] * kVec;
-            const uint4 v = load_vector<T, ALIGNED>(row, first, end, a.vocab);
+            const uint4 v = i < kNotes ? sh.note[i] : load_vector<T, ALIGNED>(row, first, end, a.vocab);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
@@ -449,11 +470,11 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) sh.warp_sum[warp] = total;
-    if (sh.count > kThreads || vectors > kList) {
+    if (sh.count > 3 * kThreads || vectors > kList) {
         const bool lost = sh.count > kList || vectors > kList;
         __syncthreads();
         if (lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
-        else trim_list(sh, k);      // more than a thread each: down to the k largest
+        else trim_list(sh, k);      // more than ranking each takes
     } else {
         __syncthreads();
     }
@@ -465,8 +486,8 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
     }
     const int n = sh.count;
     Key* out = p.lists + part * k;
-    if (tid < n) {
-        const Key mine = sh.list[tid];
+    for (int i = tid; i < n; i += kThreads) {
+        const Key mine = sh.list[i];
         const int rank = larger_than(mine, sh.list, n);
         if (rank < k) out[rank] = mine;
     }
@@ -483,120 +504,155 @@ __device__ __forceinline__ double unordered(Key u) { return __longlong_as_double
 // All lists of a group, by the CTA that finished its last chunk.
 __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     const wuda_beam_select_args& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k, chunks = p.chunks;
+    const int tid = threadIdx.x, lane = tid & 31, k = a.k, chunks = p.chunks;
     const int per_beam = chunks * k, lists = a.width * chunks, entries = lists * k;
-    // the lists' keys are on their way while the beams' sums are added
+    const float by_beam = 1.f / per_beam;
+    const auto beam_of = [&](int e) { return static_cast<int>((e + 0.5f) * by_beam); };      // e / per_beam: exact for e < kEntries
+    // ---- everything there is to read, then the beams' sums, eight lanes each
     const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
-    Key mine[kList / kThreads];
+    const Partial* partials = p.partials + static_cast<int64_t>(g) * lists;
+    Key key[kEntries / kThreads];
+    float ref[kMostLists / kThreads], score = 0.f;
+    double sum[kMostLists / kThreads];
+    bool ended = false;
 #pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) mine[i] = i * kThreads + tid < entries ? __ldcg(keys + i * kThreads + tid) : 0;
-    for (int w = warp; w < a.width; w += kWarps) {
-        const int row = g * a.width + w;
-        const float score = a.scores[row];
-        const bool dead = !(fabsf(score) < INFINITY), done = !dead && a.finished && a.finished[row];
-        double lse = 0;
-        if (!dead && !done) {
-            const Partial* parts = p.partials + static_cast<int64_t>(row) * chunks;
-            float ref[kMostChunks / 32], most = -FLT_MAX;
-            double sum[kMostChunks / 32], total = 0;
+    for (int i = 0; i < kEntries / kThreads; ++i)
+        if (i * kThreads < entries) key[i] = i * kThreads + tid < entries ? __ldcg(keys + i * kThreads + tid) : 0;
 #pragma unroll
-            for (int i = 0; i < kMostChunks / 32; ++i) {
-                const int at = i * 32 + lane;
-                ref[i] = at < chunks ? __ldcg(&parts[at].ref) : -FLT_MAX;
-                sum[i] = at < chunks ? __ldcg(&parts[at].sum) : 0;
-                most = fmaxf(most, ref[i]);
-            }
+    for (int i = 0; i < kMostLists / kThreads; ++i)
+        if (i * kThreads + tid < lists) ref[i] = __ldcg(&partials[i * kThreads + tid].ref), sum[i] = __ldcg(&partials[i * kThreads + tid].sum);
+    if (tid < a.width) {
+        score = a.scores[g * a.width + tid];
+        ended = a.finished && a.finished[g * a.width + tid];
+    }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int i = 0; i < kEntries / kThreads; ++i)
+        if (i * kThreads + tid < entries) sh.entry[i * kThreads + tid] = key[i];
 #pragma unroll
-            for (int i = 0; i < kMostChunks / 32; ++i) total += sum[i] * exp(static_cast<double>(ref[i]) - most);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            lse = most + log(total);
-        }
-        if (lane == 0) sh.lse[w] = lse, sh.score[w] = score, sh.kind[w] = dead ? 2 : done;
+    for (int i = 0; i < kMostLists / kThreads; ++i)
+        if (i * kThreads + tid < lists) sh.ref[i * kThreads + tid] = ref[i], sh.sum[i * kThreads + tid] = sum[i];
+    if (tid < a.width) {
+        sh.kind[tid] = !(fabsf(score) < INFINITY) ? 2 : ended;
+        sh.score[tid] = score;
     }
     if (tid == 0) sh.survivors = sh.there = 0, sh.least = 0;
     __syncthreads();
-    // values as ordered words; the first `deep` of every list also side by side
-    const int deep = (k + lists - 1) / lists, pool = lists * deep;
+    for (int w0 = 0; w0 < a.width; w0 += kThreads / 8) {
+        const int w = w0 + tid / 8, at = min(w, a.width - 1) * chunks;
+        float most = -FLT_MAX;
+        for (int i = lane & 7; i < chunks; i += 8) most = fmaxf(most, sh.ref[at + i]);
 #pragma unroll
-    for (int i = 0; i < kList / kThreads; ++i) {
-        const int e = i * kThreads + tid;
-        if (e >= entries) break;
-        const int list = e / k, w = list / chunks;
-        Key v = 0;
-        if (sh.kind[w] == 0) {
-            if (mine[i]) v = ordered((sh.score[w] + unordered(static_cast<uint32_t>(mine[i] >> 32))) - sh.lse[w]);
-        } else if (sh.kind[w] == 1 && e == w * per_beam) {
-            v = ordered(sh.score[w]);
-            mine[i] = key_of(0.f, static_cast<uint32_t>(a.eos_token));
-        }
-        sh.list[e] = mine[i];
-        sh.value[e] = v;
-        if (e - list * k < deep) sh.front[list * deep + e - list * k] = v;
+        for (int o = 4; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        double total = 0;
+        for (int i = lane & 7; i < chunks; i += 8) total += sh.sum[at + i] * exp2_approx((sh.ref[at + i] - most) * kLog2e);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (w < a.width && (lane & 7) == 0) sh.lse[w] = most + log(total);      // (of a beam that was not read: not used)
     }
     __syncthreads();
-    // the k-th largest of the front: nothing below it is among the k best
+    // ---- values as ordered words (0 none), in 64 bits where they are compared, in 32 where they are only bounded
+    const auto value = [&](int e) -> Key {
+        const Key key = sh.entry[e];
+        const int w = beam_of(e);
+        if (sh.kind[w] == 1) return e == w * per_beam ? ordered(sh.score[w]) : 0;
+        return sh.kind[w] == 0 && key ? ordered((sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w]) : 0;
+    };
+    const auto rounded = [](Key v) { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
+    // the first `deep` of every list, at least k of them, better 4 k: the bound is then close to the k-th value
+    const int deep = min(k, (4 * k + lists - 1) / lists), pool = lists * deep;
     for (int i = tid; i < pool; i += kThreads) {
-        const Key v = sh.front[i];
+        const int list = deep == 1 ? i : i / deep;
+        sh.front[i] = rounded(value(list * k + i - list * deep));
+    }
+    __syncthreads();
+    for (int i = tid; i < pool; i += kThreads) {      // the k-th largest of them: nothing below it is among the k best
+        const uint32_t v = sh.front[i];
         int larger = 0, not_smaller = 0, j = 0;
 #pragma unroll 4
-        for (; j + 1 < pool; j += 2) {
-            const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.front[j]);
-            larger += (other.x > v) + (other.y > v);
-            not_smaller += (other.x >= v) + (other.y >= v);
+        for (; j + 3 < pool; j += 4) {
+            const uint4 other = *reinterpret_cast<const uint4*>(&sh.front[j]);
+            larger += (other.x > v) + (other.y > v) + (other.z > v) + (other.w > v);
+            not_smaller += (other.x >= v) + (other.y >= v) + (other.z >= v) + (other.w >= v);
         }
-        if (j < pool) larger += sh.front[j] > v, not_smaller += sh.front[j] >= v;
+        for (; j < pool; ++j) larger += sh.front[j] > v, not_smaller += sh.front[j] >= v;
         if (larger < k && k <= not_smaller) sh.least = v;
     }
     __syncthreads();
-    const Key least = max(sh.least, 1ull);
-    // (the front's places are free now: the values that pass, side by side)
-    for (int e = tid; e < entries; e += kThreads)
-        if (sh.value[e] >= least) sh.passed[atomicAdd(&sh.survivors, 1)] = static_cast<uint16_t>(e);
-    __syncthreads();
-    const int n = sh.survivors;
-    const bool few = n <= kFront;
-    if (few)
-        for (int i = tid; i < n; i += kThreads) sh.front[i] = sh.value[sh.passed[i]];
-    __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-        const int e = sh.passed[i], w = e / per_beam;
-        const Key v = sh.value[e];
-        int rank = 0, equal = 0;
-        if (few) {
-            int j = 0;
+    const uint32_t least = max(sh.least, 1u);
 #pragma unroll 4
-            for (; j + 1 < n; j += 2) {
-                const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.front[j]);
-                rank += (other.x > v) + (other.y > v);
-                equal += (other.x == v) + (other.y == v);
-            }
-            if (j < n) rank += sh.front[j] > v, equal += sh.front[j] == v;
-        } else {
-            for (int j = 0; j < n; ++j) {
-                const Key other = sh.value[sh.passed[j]];
-                rank += other > v;
-                equal += other == v;
-            }
+    for (int e = tid; e < entries; e += kThreads) {
+        const Key v = value(e);
+        if (rounded(v) < least) continue;
+        const int at = atomicAdd(&sh.survivors, 1);
+        sh.passed[at] = static_cast<uint16_t>(e);
+        if (at < kFew) sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(beam_of(e));
+    }
+    __syncthreads();
+    int n = sh.survivors;
+    if (n > kFew) {
+        // many equal values: the k best by value, then by beam, then by logit and token
+        const auto mine = [&](const auto& f) {
+            for (int i = tid; i < n; i += kThreads) f(static_cast<int>(sh.passed[i]));
+        };
+        const Key worst = kth_largest(k, 64, sh.hits, [&](const auto& f) { mine([&](int e) { f(value(e)); }); });
+        const auto count = [&](const auto& test) {
+            int c = 0;
+            mine([&](int e) { c += test(e); });
+            if (tid == 0) sh.hits[0] = sh.hits[1] = 0;
+            __syncthreads();
+            return block_total(c, sh.hits, 0);
+        };
+        int wanted = k - count([&](int e) { return value(e) > worst; });
+        const int beam = 31 - static_cast<int>(kth_largest(wanted, 5, sh.hits, [&](const auto& f) {
+            mine([&](int e) { if (value(e) == worst) f(static_cast<Key>(31 - beam_of(e))); });
+        }));
+        wanted -= count([&](int e) { return value(e) == worst && beam_of(e) < beam; });
+        const Key last = kth_largest(wanted, 64, sh.hits, [&](const auto& f) {
+            mine([&](int e) { if (value(e) == worst && beam_of(e) == beam) f(sh.entry[e]); });
+        });
+        if (tid == 0) sh.survivors = 0;
+        __syncthreads();
+        for (int e = tid; e < entries; e += kThreads) {
+            const Key v = value(e);
+            const int w = beam_of(e);
+            if (v == 0 || v < worst || (v == worst && (w > beam || (w == beam && sh.entry[e] < last)))) continue;
+            const int at = atomicAdd(&sh.survivors, 1);
+            if (at < kFew) sh.passed[at] = static_cast<uint16_t>(e), sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(w);
+        }
+        __syncthreads();
+        n = min(sh.survivors, kFew);
+    }
+    // their order: larger value, lower beam; within a beam larger logit, lower token
+    for (int i = tid; i < n; i += kThreads) {
+        const Key v = sh.value[i], key = sh.entry[sh.passed[i]];
+        const int w = sh.beam[i];
+        const auto before = [&](int j) { return sh.beam[j] != w ? sh.beam[j] < w : sh.entry[sh.passed[j]] > key; };
+        int rank = 0, equal = 0, j = 0;
+        unsigned long long ties = 0;      // among the first 64
+#pragma unroll 4
+        for (; j + 1 < n; j += 2) {
+            const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.value[j]);
+            rank += (other.x > v) + (other.y > v);
+            equal += (other.x == v) + (other.y == v);
+            if (j < 64) ties |= static_cast<unsigned long long>((other.x == v) | (other.y == v) << 1) << j;
+        }
+        if (j < n) {
+            rank += sh.value[j] > v, equal += sh.value[j] == v;
+            if (j < 64) ties |= static_cast<unsigned long long>(sh.value[j] == v) << j;
+        }
+        if (equal > 1) {
+            for (; ties; ties &= ties - 1) rank += before(__ffsll(ties) - 1);
+            for (j = 64; j < n; ++j) rank += sh.value[j] == v && before(j);
         }
         if (rank >= k) continue;
-        if (equal > 1) {      // lower beam; within a beam larger logit, lower token
-            const Key key = sh.list[e];
-            for (int j = 0; j < n; ++j) {
-                const int o = sh.passed[j], ow = o / per_beam;
-                if (sh.value[o] == v && o != e) rank += ow != w ? ow < w : sh.list[o] > key;
-            }
-            if (rank >= k) continue;
-        }
         atomicAdd(&sh.there, 1);
         const int64_t at = static_cast<int64_t>(g) * k + rank;
-        const int token = static_cast<int>(token_of(sh.list[e]));
+        const bool done = sh.kind[w] == 1;
+        const int token = done ? a.eos_token : static_cast<int>(token_of(key));
         a.scores_out[at] = static_cast<float>(unordered(v));
         a.parents_out[at] = w;
         a.tokens_out[at] = token;
-        a.finished_out[at] = sh.kind[w] == 1 || token == a.eos_token;
+        a.finished_out[at] = done || token == a.eos_token;
     }
     __syncthreads();
     for (int j = sh.there + tid; j < k; j += kThreads) {
@@ -608,18 +664,15 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) beam_select_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 7) beam_select_kernel(const __grid_constant__ Params p) {
     __shared__ Shared sh;
     const wuda_beam_select_args& a = p.a;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int number = blockIdx.x % p.chunks, row = blockIdx.x / p.chunks, g = row / a.width;
-    const float score = a.scores[row];
-    if (fabsf(score) < INFINITY && !(a.finished && a.finished[row])) {
-        const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
-        if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) chunk<T, true>(sh, p, x, row, number);
-        else chunk<T, false>(sh, p, x, row, number);
-    }
+    const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) chunk<T, true>(sh, p, x, row, number);
+    else chunk<T, false>(sh, p, x, row, number);
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -635,12 +688,12 @@ __global__ void __launch_bounds__(kThreads, 3) beam_select_kernel(const __grid_c
 // Chunks of a row: enough CTAs for the device and whole rounds of loads for each, and lists that the merge can hold.
 void cut(int groups, int width, int vocab, int k, int type, int* chunks, int* chunk_vectors) {
     const int vec = type == 2 ? 4 : 8, rows = groups * width;
-    const int blocks = (vocab + vec * kThreads - 1) / (vec * kThreads);      // rounds of one load per thread
-    int n = (kCtas + rows - 1) / rows;
-    n = std::min(std::min(n, blocks), std::min(std::min(kMostChunks, kMostLists / width), kList / (width * k)));
-    const int per = (blocks + n - 1) / n;
-    *chunks = (blocks + per - 1) / per;
-    *chunk_vectors = per * kThreads;
+    const int tile = vec * kThreads * kVectors, tiles = (vocab + tile - 1) / tile;
+    int n = std::max(kCtas / rows, 1);
+    n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
+    const int per = (tiles + n - 1) / n;
+    *chunks = (tiles + per - 1) / per;
+    *chunk_vectors = per * kThreads * kVectors;
 }
 
 bool sizes_fit(int groups, int width, int vocab, int k, int type) {
