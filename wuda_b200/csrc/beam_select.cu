@@ -31,8 +31,6 @@
 namespace wuda {
 namespace beams {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
 constexpr int kVectors = 4;                 // 16-byte loads per thread and tile
 constexpr int kMostK = 64, kMostWidth = 32, kMostGroups = 256;
 constexpr int kList = 1024;                 // candidates that a chunk's CTA holds, and vectors with candidates that it notes
@@ -40,9 +38,9 @@ constexpr int kNotes = 384;                 // ... of which it keeps the content
 constexpr int kEntries = 2048;              // candidates of all chunks of a group
 constexpr int kMostChunks = 64;
 constexpr int kMostLists = 256;             // of a group
-constexpr int kFront = kMostLists + 4 * kMostK; // the lists' first candidates
 constexpr int kFew = 256;                   // values that are ranked side by side
-constexpr int kCtas = 1036;                 // CTAs of a launch: seven per SM, all at the same time
+constexpr int kCtas = 1036;                 // CTAs of 128 threads in a launch: seven per SM, all at the same time
+constexpr int kFewCtas = 148, kFewTiles = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
 
@@ -187,10 +185,22 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit typ
     else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
     else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
+// a word that grows with the value; 0 is below every number
+__device__ __forceinline__ Key ordered(double x) {
+    const long long b = __double_as_longlong(x);
+    return static_cast<Key>(b) ^ (static_cast<Key>(b >> 63) | (1ull << 63));
+}
+__device__ __forceinline__ double unordered(Key u) { return __longlong_as_double(u & (1ull << 63) ? u ^ (1ull << 63) : ~u); }
+
+// The work of a CTA of kThreads threads
+template <int kThreads>
+struct Block {
+static constexpr int kWarps = kThreads / 32;
+
 struct Shared {
     int count, vectors;                     // candidates, and vectors that may hold some (those beyond kList are lost)
     float bound;                            // the k-th largest logit so far, or less
-    int hits[2];
+    int hits[3];
     float warp_ref[kWarps];
     double warp_sum[kWarps];
     bool last;
@@ -198,26 +208,26 @@ struct Shared {
         struct {                            // a chunk
             alignas(16) Key list[kList];
             alignas(16) uint4 note[kNotes];
-            alignas(16) float part_max[kThreads];      // maxima of parts of the tiles
+            alignas(16) float part_max[128];           // maxima of parts of the tiles
             int vector[kList];                         // vectors with a logit beyond the bound of their tile
         };
         struct {                            // a group's lists
             alignas(16) Key entry[kEntries];
             alignas(16) Key value[kFew];
-            alignas(16) uint32_t front[kFront];        // values of the lists' first candidates, as ordered words
+            alignas(16) uint32_t front[128];           // largest values of shares of the lists' first candidates, as ordered words
             double sum[kMostLists], lse[kMostWidth], score[kMostWidth];
             float ref[kMostLists];
             int kind[kMostWidth];                      // 0 live, 1 finished, 2 dead
             uint16_t passed[kEntries];
             uint8_t beam[kFew];
-            uint32_t least;
+            uint32_t least, top, low[kMostWidth];
             int survivors, there;
         };
     };
 };
 
 // How many of n keys are larger, two at a time.
-__device__ __forceinline__ int larger_than(Key mine, const Key* keys, int n) {
+static __device__ __forceinline__ int larger_than(Key mine, const Key* keys, int n) {
     int rank = 0, i = 0;
 #pragma unroll 4
     for (; i + 1 < n; i += 2) {
@@ -228,24 +238,28 @@ __device__ __forceinline__ int larger_than(Key mine, const Key* keys, int n) {
     return rank;
 }
 
-__device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
+// Sum over the block, in turn `turn` of a sequence: three counters in rotation need one barrier per turn.
+static __device__ __forceinline__ int block_total(int mine, int* hits, int turn) {
     const int n = __reduce_add_sync(0xffffffffu, mine);
-    if ((threadIdx.x & 31) == 0 && n) atomicAdd(&hits[turn], n);
+    if ((threadIdx.x & 31) == 0 && n) atomicAdd(&hits[turn % 3], n);
+    if (threadIdx.x == 0) hits[(turn + 1) % 3] = 0;
     __syncthreads();
-    const int total = hits[turn];
-    if (threadIdx.x == 0) hits[turn ^ 1] = 0;      // (the other one was read before this barrier)
+    return hits[turn % 3];
+}
+static __device__ __forceinline__ void start_totals(int* hits) {
     __syncthreads();
-    return total;
+    if (threadIdx.x < 3) hits[threadIdx.x] = 0;
+    __syncthreads();
 }
 
-// The largest K such that at least `want` of the block's keys are at or above it, bit by bit from `bits` down; 0 where they are fewer.
-// each(f) calls f(key) for every key of the thread.  All threads; ends behind a barrier.
+// The largest K such that at least `want` of the block's keys are at or above it, bit by bit; low <= K <= high is known (0 and ~0 where
+// nothing is; low counts where they are fewer than `want`).  each(f) calls f(key) for every key of the thread.  All threads.
 template <typename Each>
-__device__ __forceinline__ Key kth_largest(int want, int bits, int* hits, const Each& each) {
-    if (threadIdx.x == 0) hits[0] = hits[1] = 0;
-    __syncthreads();
-    Key least = 0;
-    for (int bit = bits - 1, turn = 0; bit >= 0; --bit, turn ^= 1) {
+static __device__ __forceinline__ Key kth_largest(int want, Key low, Key high, int* hits, const Each& each) {
+    start_totals(hits);
+    int bit = 63 - __clzll(low ^ high);      // (-1: they are equal)
+    Key least = bit < 63 ? low & ~((2ull << bit) - 1) : 0;
+    for (int turn = 0; bit >= 0; --bit, ++turn) {
         const Key probe = least | (1ull << bit);
         int mine = 0;
         each([&](Key key) { mine += key >= probe; });
@@ -259,7 +273,7 @@ __device__ __forceinline__ Key kth_largest(int want, int bits, int* hits, const 
 // The k largest of the list and of the tile's keys (unique ones, 0 none) become the list, or all of them where they are fewer.  Returns
 // the k-th.  All threads; ends behind a barrier.
 template <int N>
-__device__ __forceinline__ Key select_exactly(Shared& sh, const Key (&tile)[N], int k) {
+static __device__ __forceinline__ Key select_exactly(Shared& sh, const Key (&tile)[N], int k) {
     Key held[kList / kThreads];
     const int count = min(sh.count, kList);
 #pragma unroll
@@ -270,7 +284,8 @@ __device__ __forceinline__ Key select_exactly(Shared& sh, const Key (&tile)[N], 
 #pragma unroll
         for (int i = 0; i < N; ++i) f(tile[i]);
     };
-    const Key least = kth_largest(k, 64, sh.hits, each);
+    const Key least = kth_largest(k, 0, ~0ull, sh.hits, each);
+    __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     each([&](Key key) {
@@ -279,7 +294,7 @@ __device__ __forceinline__ Key select_exactly(Shared& sh, const Key (&tile)[N], 
     __syncthreads();
     return least;
 }
-__device__ __noinline__ void trim_list(Shared& sh, int k) {
+static __device__ __noinline__ void trim_list(Shared& sh, int k) {
     const Key none[1] = {0};
     select_exactly(sh, none, k);
 }
@@ -287,7 +302,7 @@ __device__ __noinline__ void trim_list(Shared& sh, int k) {
 // A chunk's k largest keys where the list overflowed (rows sorted upwards, rows of one value, rows masked but for their end): tile by tile with
 // exact selections, as far as a tile has a key above the k-th largest so far.
 template <typename T>
-__device__ __noinline__ void candidates_exactly(Shared& sh, const T* row, int c0, int end, int vocab, int k) {
+static __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row, int c0, int end, int vocab, int k) {
     constexpr int kVec = Type<T>::kVec;
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
@@ -313,27 +328,30 @@ __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row, int c0
     }
 }
 
-// The k-th largest of the maxima that the threads (k <= 32: pairs of them) have seen: k logits so far are at or above it.
-__device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
-    const int tid = threadIdx.x;
-    const bool pairs = k <= 32;
-    const float part = pairs ? fmaxf(so_far, __shfl_xor_sync(0xffffffffu, so_far, 1)) : so_far;
-    if (!pairs || tid % 2 == 0) sh.part_max[pairs ? tid / 2 : tid] = part;
+// The k-th largest of 64 (k <= 32) or 128 maxima, of as many groups of neighbouring threads over all that they have seen: k logits so
+// far are at or above it.
+static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
+    const int tid = threadIdx.x, parts = k <= 32 ? 64 : 128, by = kThreads / parts;
+    float part = so_far;
+#pragma unroll
+    for (int o = 1; o < kThreads / 64; o <<= 1)
+        if (o < by) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, o));
+    if (tid % by == 0) sh.part_max[tid / by] = part;
     __syncthreads();
-    int larger = 0, not_smaller = 0;      // than the thread's own part; each of a pair of threads counts half of them
-    const int n = pairs ? kThreads / 16 : kThreads / 4;
-    const float4* parts = reinterpret_cast<const float4*>(sh.part_max) + (pairs ? tid % 2 * n : 0);
+    int larger = 0, not_smaller = 0;      // than the group's maximum; each of its threads counts a share of them
+    const int n = parts / 4 / by;
+    const float4* share = reinterpret_cast<const float4*>(sh.part_max) + tid % by * n;
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
-        const float4 other = parts[i];
+        const float4 other = share[i];
         larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
         not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
     }
-    if (pairs) {
-        larger += __shfl_xor_sync(0xffffffffu, larger, 1);
-        not_smaller += __shfl_xor_sync(0xffffffffu, not_smaller, 1);
-    }
-    if (larger < k && k <= not_smaller) sh.bound = part;      // (equal ones write the same)
+    int both = larger | not_smaller << 16;
+#pragma unroll
+    for (int o = 1; o < kThreads / 64; o <<= 1)
+        if (o < by) both += __shfl_xor_sync(0xffffffffu, both, o);
+    if ((both & 0xffff) < k && k <= both >> 16) sh.bound = part;      // (equal ones write the same)
     __syncthreads();
     *raised = sh.bound > bound;
     return sh.bound;
@@ -341,7 +359,7 @@ __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, fl
 
 // A chunk of a row: its partial sum, and its k largest keys in descending order.
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row, int row_number, int number) {
+static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row, int row_number, int number) {
     constexpr int kVec = Type<T>::kVec;
     const wuda_beam_select_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
@@ -494,15 +512,8 @@ __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const T* row,
     if (tid >= n && tid < k) out[tid] = 0;
 }
 
-// a word that grows with the value; 0 is below every number
-__device__ __forceinline__ Key ordered(double x) {
-    const long long b = __double_as_longlong(x);
-    return static_cast<Key>(b) ^ (static_cast<Key>(b >> 63) | (1ull << 63));
-}
-__device__ __forceinline__ double unordered(Key u) { return __longlong_as_double(u & (1ull << 63) ? u ^ (1ull << 63) : ~u); }
-
 // All lists of a group, by the CTA that finished its last chunk.
-__device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
+static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     const wuda_beam_select_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, k = a.k, chunks = p.chunks;
     const int per_beam = chunks * k, lists = a.width * chunks, entries = lists * k;
@@ -512,14 +523,15 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
     const Partial* partials = p.partials + static_cast<int64_t>(g) * lists;
     Key key[kEntries / kThreads];
-    float ref[kMostLists / kThreads], score = 0.f;
-    double sum[kMostLists / kThreads];
+    constexpr int kParts = (kMostLists + kThreads - 1) / kThreads;
+    float ref[kParts], score = 0.f;
+    double sum[kParts];
     bool ended = false;
 #pragma unroll
     for (int i = 0; i < kEntries / kThreads; ++i)
         if (i * kThreads < entries) key[i] = i * kThreads + tid < entries ? __ldcg(keys + i * kThreads + tid) : 0;
 #pragma unroll
-    for (int i = 0; i < kMostLists / kThreads; ++i)
+    for (int i = 0; i < kParts; ++i)
         if (i * kThreads + tid < lists) ref[i] = __ldcg(&partials[i * kThreads + tid].ref), sum[i] = __ldcg(&partials[i * kThreads + tid].sum);
     if (tid < a.width) {
         score = a.scores[g * a.width + tid];
@@ -529,7 +541,7 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     for (int i = 0; i < kEntries / kThreads; ++i)
         if (i * kThreads + tid < entries) sh.entry[i * kThreads + tid] = key[i];
 #pragma unroll
-    for (int i = 0; i < kMostLists / kThreads; ++i)
+    for (int i = 0; i < kParts; ++i)
         if (i * kThreads + tid < lists) sh.ref[i * kThreads + tid] = ref[i], sh.sum[i * kThreads + tid] = sum[i];
     if (tid < a.width) {
         sh.kind[tid] = !(fabsf(score) < INFINITY) ? 2 : ended;
@@ -557,57 +569,98 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         if (sh.kind[w] == 1) return e == w * per_beam ? ordered(sh.score[w]) : 0;
         return sh.kind[w] == 0 && key ? ordered((sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w]) : 0;
     };
-    const auto rounded = [](Key v) { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
+    const auto rounded = [](Key v) -> uint32_t { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
     // the first `deep` of every list, at least k of them, better 4 k: the bound is then close to the k-th value
     const int deep = min(k, (4 * k + lists - 1) / lists), pool = lists * deep;
+    uint32_t part = 0;      // the largest of a thread's share: 128 or more of them are at least 2 k
     for (int i = tid; i < pool; i += kThreads) {
         const int list = deep == 1 ? i : i / deep;
-        sh.front[i] = rounded(value(list * k + i - list * deep));
+        part = max(part, rounded(value(list * k + i - list * deep)));
     }
+    if constexpr (kThreads > 128) {
+#pragma unroll
+        for (int o = 1; o < kThreads / 128; o <<= 1) part = max(part, __shfl_xor_sync(0xffffffffu, part, o));
+    }
+    if (tid % (kThreads / 128) == 0) sh.front[tid / (kThreads / 128)] = part;
     __syncthreads();
-    for (int i = tid; i < pool; i += kThreads) {      // the k-th largest of them: nothing below it is among the k best
-        const uint32_t v = sh.front[i];
-        int larger = 0, not_smaller = 0, j = 0;
-#pragma unroll 4
-        for (; j + 3 < pool; j += 4) {
-            const uint4 other = *reinterpret_cast<const uint4*>(&sh.front[j]);
-            larger += (other.x > v) + (other.y > v) + (other.z > v) + (other.w > v);
-            not_smaller += (other.x >= v) + (other.y >= v) + (other.z >= v) + (other.w >= v);
+    // the k-th largest of them: nothing below it is among the k best
+    if (tid % (kThreads / 128) == 0) {
+        int larger = 0, not_smaller = 0;
+#pragma unroll 8
+        for (int i = 0; i < 128; i += 4) {
+            const uint4 other = *reinterpret_cast<const uint4*>(&sh.front[i]);
+            larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
+            not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
         }
-        for (; j < pool; ++j) larger += sh.front[j] > v, not_smaller += sh.front[j] >= v;
-        if (larger < k && k <= not_smaller) sh.least = v;
+        if (larger < k && k <= not_smaller) sh.least = part;
+        if (larger == 0) sh.top = part;
     }
     __syncthreads();
     const uint32_t least = max(sh.least, 1u);
+    // the bound as a logit of each beam, a little lower (what is compared with it is rounded in other places)
+    if (tid < a.width) {
+        const double logit = unordered(least) - sh.score[tid] + sh.lse[tid];
+        const float low = static_cast<float>(logit - 1e-6 * (fabs(logit) + fabs(sh.score[tid]) + fabs(sh.lse[tid])));
+        sh.low[tid] = sh.kind[tid] == 0 ? (least > 1u && low == low ? ordered(low) : 1u) : sh.kind[tid] == 1 ? 0u : 0xffffffffu;
+    }
+    __syncthreads();
 #pragma unroll 4
     for (int e = tid; e < entries; e += kThreads) {
+        const int w = beam_of(e);
+        if (static_cast<uint32_t>(sh.entry[e] >> 32) < sh.low[w]) continue;
         const Key v = value(e);
         if (rounded(v) < least) continue;
         const int at = atomicAdd(&sh.survivors, 1);
         sh.passed[at] = static_cast<uint16_t>(e);
-        if (at < kFew) sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(beam_of(e));
+        if (at < kFew) sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(w);
     }
     __syncthreads();
     int n = sh.survivors;
+    if (n > 2 * k + 32) {
+        // a few beams have most of the best: the k-th largest value of what passed, exactly but for its rounding
+        uint32_t mine[kEntries / kThreads];
+#pragma unroll
+        for (int i = 0; i < kEntries / kThreads; ++i)
+            if (i * kThreads < n) mine[i] = i * kThreads + tid < n ? rounded(value(sh.passed[i * kThreads + tid])) : 0;
+        const uint32_t bound = static_cast<uint32_t>(kth_largest(k, least, sh.top, sh.hits, [&](const auto& f) {
+#pragma unroll
+            for (int i = 0; i < kEntries / kThreads; ++i)
+                if (i * kThreads < n) f(static_cast<Key>(mine[i]));
+        }));
+        uint16_t entry[kEntries / kThreads];
+#pragma unroll
+        for (int i = 0; i < kEntries / kThreads; ++i)
+            if (i * kThreads + tid < n) entry[i] = sh.passed[i * kThreads + tid];
+        if (tid == 0) sh.survivors = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEntries / kThreads; ++i) {
+            if (i * kThreads + tid >= n || mine[i] < bound) continue;
+            const int at = atomicAdd(&sh.survivors, 1);
+            sh.passed[at] = entry[i];
+            if (at < kFew) sh.value[at] = value(entry[i]), sh.beam[at] = static_cast<uint8_t>(beam_of(entry[i]));
+        }
+        __syncthreads();
+        n = sh.survivors;
+    }
     if (n > kFew) {
         // many equal values: the k best by value, then by beam, then by logit and token
         const auto mine = [&](const auto& f) {
             for (int i = tid; i < n; i += kThreads) f(static_cast<int>(sh.passed[i]));
         };
-        const Key worst = kth_largest(k, 64, sh.hits, [&](const auto& f) { mine([&](int e) { f(value(e)); }); });
+        const Key worst = kth_largest(k, 0, ~0ull, sh.hits, [&](const auto& f) { mine([&](int e) { f(value(e)); }); });
         const auto count = [&](const auto& test) {
             int c = 0;
             mine([&](int e) { c += test(e); });
-            if (tid == 0) sh.hits[0] = sh.hits[1] = 0;
-            __syncthreads();
+            start_totals(sh.hits);
             return block_total(c, sh.hits, 0);
         };
         int wanted = k - count([&](int e) { return value(e) > worst; });
-        const int beam = 31 - static_cast<int>(kth_largest(wanted, 5, sh.hits, [&](const auto& f) {
+        const int beam = 31 - static_cast<int>(kth_largest(wanted, 0, 31, sh.hits, [&](const auto& f) {
             mine([&](int e) { if (value(e) == worst) f(static_cast<Key>(31 - beam_of(e))); });
         }));
         wanted -= count([&](int e) { return value(e) == worst && beam_of(e) < beam; });
-        const Key last = kth_largest(wanted, 64, sh.hits, [&](const auto& f) {
+        const Key last = kth_largest(wanted, 0, ~0ull, sh.hits, [&](const auto& f) {
             mine([&](int e) { if (value(e) == worst && beam_of(e) == beam) f(sh.entry[e]); });
         });
         if (tid == 0) sh.survivors = 0;
@@ -628,20 +681,24 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         const int w = sh.beam[i];
         const auto before = [&](int j) { return sh.beam[j] != w ? sh.beam[j] < w : sh.entry[sh.passed[j]] > key; };
         int rank = 0, equal = 0, j = 0;
-        unsigned long long ties = 0;      // among the first 64
+        uint32_t ties[2] = {0, 0};      // among the first 64
 #pragma unroll 4
         for (; j + 1 < n; j += 2) {
             const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.value[j]);
             rank += (other.x > v) + (other.y > v);
-            equal += (other.x == v) + (other.y == v);
-            if (j < 64) ties |= static_cast<unsigned long long>((other.x == v) | (other.y == v) << 1) << j;
+            const uint32_t same = (other.x == v) | (other.y == v) << 1;
+            equal += __popc(same);
+            if (j < 64) ties[0] |= j < 32 ? same << j : 0, ties[1] |= j < 32 ? 0 : same << (j - 32);
         }
         if (j < n) {
-            rank += sh.value[j] > v, equal += sh.value[j] == v;
-            if (j < 64) ties |= static_cast<unsigned long long>(sh.value[j] == v) << j;
+            const uint32_t same = sh.value[j] == v;
+            rank += sh.value[j] > v, equal += same;
+            if (j < 64) ties[0] |= j < 32 ? same << j : 0, ties[1] |= j < 32 ? 0 : same << (j - 32);
         }
         if (equal > 1) {
-            for (; ties; ties &= ties - 1) rank += before(__ffsll(ties) - 1);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                for (uint32_t m = ties[t]; m; m &= m - 1) rank += before(t * 32 + __ffs(m) - 1);
             for (j = 64; j < n; ++j) rank += sh.value[j] == v && before(j);
         }
         if (rank >= k) continue;
@@ -662,17 +719,19 @@ __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         a.finished_out[at] = 0;
     }
 }
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 7) beam_select_kernel(const __grid_constant__ Params p) {
-    __shared__ Shared sh;
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(const __grid_constant__ Params p) {
+    using B = Block<kThreads>;
+    __shared__ typename B::Shared sh;
     const wuda_beam_select_args& a = p.a;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int number = blockIdx.x % p.chunks, row = blockIdx.x / p.chunks, g = row / a.width;
     const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
-    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) chunk<T, true>(sh, p, x, row, number);
-    else chunk<T, false>(sh, p, x, row, number);
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) B::template chunk<T, true>(sh, p, x, row, number);
+    else B::template chunk<T, false>(sh, p, x, row, number);
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -682,18 +741,26 @@ __global__ void __launch_bounds__(kThreads, 7) beam_select_kernel(const __grid_c
     __syncthreads();
     if (!sh.last) return;
     __threadfence();
-    merge(sh, p, g);
+    B::merge(sh, p, g);
 }
 
-// Chunks of a row: enough CTAs for the device and whole rounds of loads for each, and lists that the merge can hold.
-void cut(int groups, int width, int vocab, int k, int type, int* chunks, int* chunk_vectors) {
-    const int vec = type == 2 ? 4 : 8, rows = groups * width;
-    const int tile = vec * kThreads * kVectors, tiles = (vocab + tile - 1) / tile;
-    int n = std::max(kCtas / rows, 1);
-    n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
-    const int per = (tiles + n - 1) / n;
-    *chunks = (tiles + per - 1) / per;
-    *chunk_vectors = per * kThreads * kVectors;
+// How the rows are cut: chunks of whole tiles, as many as CTAs of 128 threads are resident on the device together, and lists that the
+// merge can hold.  Where that leaves less than a warp per scheduler and several tiles per CTA, CTAs of 512 threads.
+struct Cut {
+    int threads, chunks, chunk_vectors;
+};
+Cut cut(int groups, int width, int vocab, int k, int type) {
+    const int rows = groups * width;
+    Cut c = {};
+    for (c.threads = 128;; c.threads = 512) {
+        const int tile = (type == 2 ? 4 : 8) * c.threads * kVectors, tiles = (vocab + tile - 1) / tile;
+        int n = std::max(kCtas / (c.threads / 128) / rows, 1);
+        n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
+        const int per = (tiles + n - 1) / n;
+        c.chunks = (tiles + per - 1) / per;
+        c.chunk_vectors = per * c.threads * kVectors;
+        if (c.threads == 512 || per < kFewTiles || rows * c.chunks >= kFewCtas) return c;
+    }
 }
 
 bool sizes_fit(int groups, int width, int vocab, int k, int type) {
@@ -708,9 +775,7 @@ extern "C" int64_t wuda_beam_select_workspace_bytes(int groups, int width, int v
     using namespace wuda::beams;
     if (!sizes_fit(groups, width, vocab, k, logits_type)) return -1;
     if (groups == 0) return 0;
-    int chunks, vectors;
-    cut(groups, width, vocab, k, logits_type, &chunks, &vectors);
-    return static_cast<int64_t>(groups) * width * chunks * (k * sizeof(Key) + sizeof(Partial));
+    return static_cast<int64_t>(groups) * width * cut(groups, width, vocab, k, logits_type).chunks * (k * sizeof(Key) + sizeof(Partial));
 }
 
 extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream) {
@@ -738,11 +803,16 @@ extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream)
     if (const int st = current_device_info(&dev)) return st;
     Params p;
     p.a = a;
-    cut(a.groups, a.width, a.vocab, a.k, a.logits_type, &p.chunks, &p.chunk_vectors);
+    const Cut c = cut(a.groups, a.width, a.vocab, a.k, a.logits_type);
+    p.chunks = c.chunks;
+    p.chunk_vectors = c.chunk_vectors;
     const int64_t parts = static_cast<int64_t>(a.groups) * a.width * p.chunks;
     p.partials = static_cast<Partial*>(a.workspace);
     p.lists = reinterpret_cast<Key*>(p.partials + parts);
-    void (*kernel)(Params) = a.logits_type == 0 ? beam_select_kernel<__nv_bfloat16> : a.logits_type == 1 ? beam_select_kernel<__half> : beam_select_kernel<float>;
-    WUDA_CUDA(launch_pdl(kernel, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), p));
+    static void (*const kernels[2][3])(Params) = {
+        {beam_select_kernel<__nv_bfloat16, 128>, beam_select_kernel<__half, 128>, beam_select_kernel<float, 128>},
+        {beam_select_kernel<__nv_bfloat16, 512>, beam_select_kernel<__half, 512>, beam_select_kernel<float, 512>}};
+    WUDA_CUDA(launch_pdl(kernels[c.threads == 512][a.logits_type], dim3(static_cast<unsigned>(parts)), dim3(c.threads), 0,
+                         static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }
