@@ -37,7 +37,7 @@ def step_tables(slots, new_tokens, lengths, idx_table, cmp_table, swa_table, idx
                     stopped, served = True, False
         if not served:
             left_out += slot != -1
-            tokens += [(0, -1, -1, -1, -1)] * max(n, 0)
+            tokens += [(0, -1, -1, -1, -1)] * min(max(n, 0), max_tokens)      # (those beyond the buffers are cut below)
             rows_out.append((0, [], [], []))
             continue
         lengths[slot] = now

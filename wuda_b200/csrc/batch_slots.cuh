@@ -10,6 +10,32 @@ namespace wuda {
 constexpr int kMostSlots = 16384;      // one word of shared memory per slot
 constexpr int kMostRows = 4096;
 
+// Division of a 32-bit number by one that the host knows: a high product, an add and two shifts instead of some thirty
+// instructions (T. Granlund and P. Montgomery, "Division by invariant integers using multiplication", figure 4.1).
+struct Divisor {
+    uint32_t by, factor;
+    int shift1, shift2;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) : by(d) {
+        int l = 0;
+        while (l < 32 && (1ull << l) < d) ++l;
+        factor = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+        shift1 = l < 1 ? l : 1;
+        shift2 = l > 1 ? l - 1 : 0;
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+        const uint32_t t = __umulhi(factor, n);
+        return (t + ((n - t) >> shift1)) >> shift2;
+    }
+    __device__ __forceinline__ uint32_t rest(uint32_t n) const { return n - quotient(n) * by; }
+    __device__ __forceinline__ uint32_t quotient_up(uint32_t n) const {      // of n / by
+        const uint32_t q = quotient(n);
+        return q + (q * by != n);
+    }
+#endif
+};
+
 #ifdef __CUDACC__
 __device__ __forceinline__ void report(int32_t* status, int code) {
     if (status) atomicCAS(status, 0, code);

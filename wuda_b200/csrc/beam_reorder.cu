@@ -13,7 +13,10 @@ namespace reorder {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPieceBytes = 16384;
+constexpr int kUnroll = 4;                   // units of a thread in flight
+constexpr int kResident = 5;                 // CTAs of an SM
+constexpr int kBatch = 32;                   // pieces that a CTA plans at a time
+constexpr int kPieceBytes = 16384;           // 16 bytes x kUnroll x kThreads
 
 struct Params {
     wuda_beam_reorder_args a;
@@ -21,12 +24,14 @@ struct Params {
     const int32_t* slots;
     int32_t* slots_out;
     int groups;
-    int state_pieces;                            // pieces of all state rows
-    int piece_entries[WUDA_BEAM_MAX_POOLS];      // entries of a page that are copied at a time, a multiple of 4
+    int state_first[WUDA_BEAM_MAX_STATES + 1];   // the first piece of each state's rows, the pieces of all
+    int state_pieces;
+    int piece_shift[WUDA_BEAM_MAX_POOLS];        // entries of a page that are copied at a time: 2 ^ this, at least 4
+    Divisor per_entry[WUDA_BEAM_MAX_POOLS], per_block[WUDA_BEAM_MAX_POOLS], per_page[WUDA_BEAM_MAX_POOLS];      // tokens, entries, pieces
     int32_t* status;
 };
 
-inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (4ull * rows + 1 + capacity); }
+inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (6ull * rows + 1 + capacity); }
 
 __device__ __forceinline__ int lowest_but(uint32_t set, int n) {      // the n-th lowest member, -1 where there are fewer
     for (; n > 0 && set; --n) set &= set - 1;
@@ -36,56 +41,85 @@ __device__ __forceinline__ int lowest_but(uint32_t set, int n) {      // the n-t
 struct Span {
     int first_page, pages, entries;      // pages [first_page, pages), entries in all pages
 };
-__device__ __forceinline__ Span span_of(const wuda_beam_pool& pool, int length, int shared) {
+__device__ __forceinline__ Span span_of(const Params& p, int pool, int length, int shared) {
+    const int ring = p.a.pools[pool].ring;
     Span s;
-    s.entries = pool.ring > 0 ? min(length / pool.tokens_per_entry, pool.ring) : length / pool.tokens_per_entry;
-    s.pages = (s.entries + pool.entries_per_block - 1) / pool.entries_per_block;
-    s.first_page = pool.ring > 0 ? 0 : min(shared / pool.tokens_per_entry / pool.entries_per_block, s.pages);
+    s.entries = static_cast<int>(p.per_entry[pool].quotient(length));
+    if (ring > 0) s.entries = min(s.entries, ring);
+    s.pages = static_cast<int>(p.per_block[pool].quotient_up(s.entries));
+    s.first_page = ring > 0 ? 0 : min(static_cast<int>(p.per_block[pool].quotient(p.per_entry[pool].quotient(shared))), s.pages);
     return s;
 }
-__device__ __forceinline__ int pieces_of(const wuda_beam_pool& pool, const Span& s, int piece_entries) {
+__device__ __forceinline__ int pieces_of(const Params& p, int pool, const Span& s) {
     if (s.first_page >= s.pages) return 0;
-    const int per_page = (pool.entries_per_block + piece_entries - 1) / piece_entries;
-    const int last = s.entries - (s.pages - 1) * pool.entries_per_block;
-    return (s.pages - 1 - s.first_page) * per_page + (last + piece_entries - 1) / piece_entries;
+    const int last = s.entries - (s.pages - 1) * p.a.pools[pool].entries_per_block;
+    return (s.pages - 1 - s.first_page) * static_cast<int>(p.per_page[pool].by) + ((last + (1 << p.piece_shift[pool]) - 1) >> p.piece_shift[pool]);
 }
 
-// bytes (a multiple of 4) from src to dst by all threads of the block; 16 at a time where both lie on 16 bytes
-__device__ __forceinline__ void copy_block(uint8_t* dst, const uint8_t* src, int64_t bytes) {
-    int64_t done = 0;
-    if (((reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src)) & 15) == 0) {
-        const int64_t n = bytes / 16;
-        for (int64_t i = threadIdx.x; i < n; i += kThreads) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(src)[i];
-        done = n * 16;
+// What one piece copies: up to two runs of bytes (multiples of 4), the second behind the first only in its number of units.
+struct Piece {
+    const uint8_t* src[2];
+    uint8_t* dst[2];
+    int bytes[2];
+};
+
+// By all threads of the block: four units in flight per thread, loads first.  A unit is 16 bytes where everything lies on 16, else 4.
+template <typename Unit>
+__device__ __forceinline__ void copy_units(const Piece& c, int n0, int n) {
+    for (int i0 = 0; i0 < n; i0 += kUnroll * kThreads) {
+        Unit v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kThreads + threadIdx.x;
+            if (i < n) v[u] = i < n0 ? __ldcs(reinterpret_cast<const Unit*>(c.src[0]) + i) : __ldcs(reinterpret_cast<const Unit*>(c.src[1]) + i - n0);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = i0 + u * kThreads + threadIdx.x;
+            if (i < n) *(i < n0 ? reinterpret_cast<Unit*>(c.dst[0]) + i : reinterpret_cast<Unit*>(c.dst[1]) + i - n0) = v[u];
+        }
     }
-    for (int64_t i = done / 4 + threadIdx.x; i < bytes / 4; i += kThreads)
-        reinterpret_cast<uint32_t*>(dst)[i] = reinterpret_cast<const uint32_t*>(src)[i];
+}
+__device__ __forceinline__ void copy_piece(const Piece& c) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(c.src[0]) | reinterpret_cast<uintptr_t>(c.dst[0]) | reinterpret_cast<uintptr_t>(c.src[1]) |
+                           reinterpret_cast<uintptr_t>(c.dst[1]) | c.bytes[0] | c.bytes[1];
+    if (bits & 15) copy_units<uint32_t>(c, c.bytes[0] / 4, (c.bytes[0] + c.bytes[1]) / 4);
+    else copy_units<uint4>(c, c.bytes[0] / 16, (c.bytes[0] + c.bytes[1]) / 16);
 }
 
-__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const __grid_constant__ Params p) {
     extern __shared__ int mem[];
     __shared__ int scan[33];
+    __shared__ Piece pieces[kBatch];
     const wuda_beam_reorder_args& a = p.a;
     const int width = a.width, rows = p.groups * width, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int* slot = mem;                 // of the beams now
-    int* source = slot + rows;       // of new beam j: the slot that its own is filled from, -1 no fork
+    int* source = slot + rows;       // of new beam j: the beam of its group that it continues; then the slot that its own is filled from, -1 no fork
     int* own = source + rows;        // of new beam j: its slot
     int* begin = own + rows;         // of new beam j: the number of its first piece
-    int* first = begin + rows + 1;   // (load_slots)
+    int* length = begin + rows + 1;  // of the beams now; then of what a fork copies
+    int* common = length + rows;     // their shared lengths
+    int* first = common + rows;      // (load_slots)
     int32_t* status = blockIdx.x == 0 ? p.status : nullptr;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int per = (rows + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, rows), b1 = min(b0 + per, rows);
+    for (int b = b0; b < b1; ++b) {
+        source[b] = p.parents[b];
+        const int s = p.slots[b];
+        const bool inside = s >= 0 && s < a.capacity;
+        length[b] = inside ? a.lengths[s] : -1;
+        common[b] = inside && a.shared_lengths ? a.shared_lengths[s] : 0;
+    }
     load_slots(p.slots, b0, b1, a.capacity, slot, first, status);
-    for (int b = b0; b < b1; ++b) source[b] = p.parents[b];
     __syncthreads();
 
     // ---- new slots and forks, a group per warp
     for (int g = warp; g < p.groups; g += kWarps) {
         const int at = g * width + lane;
         const bool mine = lane < width;
-        const int now = mine ? slot[at] : -1;
+        const int now = mine ? slot[at] : -1, tokens = mine ? length[at] : -1, shared = mine ? common[at] : 0;
         int parent = mine ? source[at] : -1;
         if (parent < -1 || parent >= width) {
             report(status, WUDA_DEV_BAD_PARENT);
@@ -104,11 +138,21 @@ __global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_con
         const int place = keeps ? parent : (parent >= 0 ? lowest_but(places, __popc(further & below))
                                                         : lowest_but(places, __popc(further) + __popc(orphans & below)));
         int to = __shfl_sync(0xffffffffu, now, max(place, 0));
+        const int to_tokens = __shfl_sync(0xffffffffu, tokens, max(place, 0)), to_shared = __shfl_sync(0xffffffffu, shared, max(place, 0));
+        const int from_tokens = __shfl_sync(0xffffffffu, tokens, max(parent, 0)), from_shared = __shfl_sync(0xffffffffu, shared, max(parent, 0));
         if (place < 0) to = -1;
+        bool fork = parent >= 0 && !keeps && to >= 0;
+        if (fork && (from_tokens < 0 || from_shared < 0 || to_tokens != from_tokens || to_shared != from_shared)) {
+            report(status, WUDA_DEV_BAD_LENGTH);
+            fork = false;
+            to = -1;
+        }
         __syncwarp();
         if (mine) {
-            source[at] = parent >= 0 && !keeps && to >= 0 ? from : -1;
+            source[at] = fork ? from : -1;
             own[at] = to;
+            length[at] = from_tokens;
+            common[at] = from_shared;
         }
     }
     __syncthreads();
@@ -118,13 +162,12 @@ __global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_con
     for (int b = b0; b < b1; ++b) {
         begin[b] = sum[0];
         if (source[b] < 0) continue;
-        const int length = a.lengths[source[b]], shared = a.shared_lengths ? a.shared_lengths[source[b]] : 0;
-        bool good = length >= 0 && shared >= 0 && a.lengths[own[b]] == length && (!a.shared_lengths || a.shared_lengths[own[b]] == shared);
+        bool good = true;
         int pieces = p.state_pieces;
         for (int i = 0; i < a.num_pools; ++i) {
-            const Span s = span_of(a.pools[i], length, shared);
+            const Span s = span_of(p, i, length[b], common[b]);
             good = good && s.pages <= a.pools[i].table_width;
-            if (good) pieces += pieces_of(a.pools[i], s, p.piece_entries[i]);
+            if (good) pieces += pieces_of(p, i, s);
         }
         if (!good) {
             report(status, WUDA_DEV_BAD_LENGTH);
@@ -140,8 +183,9 @@ __global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_con
     }
     __syncthreads();
 
-    // ---- the copies
-    for (int unit = blockIdx.x; unit < total[0]; unit += gridDim.x) {
+    // ---- the copies.  What a piece is takes divisions and two dependent loads: a thread per piece works that out for the CTA's next kBatch.
+    const auto piece_of = [&](int unit) {
+        Piece c = {};
         int b = 0;       // the last beam whose pieces start at or before this one: the fork that it belongs to
         for (int lo = 0, hi = rows; lo < hi;) {
             const int mid = (lo + hi) >> 1;
@@ -151,48 +195,51 @@ __global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_con
         const int src = source[b], dst = own[b];
         int piece = unit - begin[b];
         if (piece < p.state_pieces) {
-            for (int i = 0; i < a.num_states; ++i) {
-                const int64_t bytes = a.states[i].row_bytes;
-                const int n = static_cast<int>((bytes + kPieceBytes - 1) / kPieceBytes);
-                if (piece < n) {
-                    const int64_t at = static_cast<int64_t>(piece) * kPieceBytes;
-                    uint8_t* data = static_cast<uint8_t*>(a.states[i].data);
-                    copy_block(data + dst * bytes + at, data + src * bytes + at, min(static_cast<int64_t>(kPieceBytes), bytes - at));
-                    break;
-                }
-                piece -= n;
-            }
-            continue;
+            int i = 0;
+            while (piece >= p.state_first[i + 1]) ++i;
+            const int64_t bytes = a.states[i].row_bytes, at = static_cast<int64_t>(piece - p.state_first[i]) * kPieceBytes;
+            uint8_t* data = static_cast<uint8_t*>(a.states[i].data);
+            c.src[0] = data + src * bytes + at, c.dst[0] = data + dst * bytes + at;
+            c.bytes[0] = static_cast<int>(min(static_cast<int64_t>(kPieceBytes), bytes - at));
+            return c;
         }
         piece -= p.state_pieces;
-        const int length = a.lengths[src], shared = a.shared_lengths ? a.shared_lengths[src] : 0;
         for (int i = 0; i < a.num_pools; ++i) {
             const wuda_beam_pool& pool = a.pools[i];
-            const Span s = span_of(pool, length, shared);
-            const int step = p.piece_entries[i], n = pieces_of(pool, s, step);
+            const Span s = span_of(p, i, length[b], common[b]);
+            const int n = pieces_of(p, i, s);
             if (piece >= n) {
                 piece -= n;
                 continue;
             }
-            const int per_page = (pool.entries_per_block + step - 1) / step;
-            const int page = s.first_page + piece / per_page, e0 = piece % per_page * step;
-            const int e1 = min(min(e0 + step, pool.entries_per_block), s.entries - page * pool.entries_per_block);
+            const int of = static_cast<int>(p.per_page[i].quotient(piece)), page = s.first_page + of;
+            const int e0 = (piece - of * static_cast<int>(p.per_page[i].by)) << p.piece_shift[i];
+            const int e1 = min(min(e0 + (1 << p.piece_shift[i]), pool.entries_per_block), s.entries - page * pool.entries_per_block);
             const int from = pool.table[static_cast<int64_t>(src) * pool.table_width + page];
             const int to = pool.table[static_cast<int64_t>(dst) * pool.table_width + page];
             if (from < 0 || from >= pool.num_blocks || to < 0 || to >= pool.num_blocks) {
                 report(p.status, WUDA_DEV_BAD_PAGE_INDEX);
-                break;
+                return c;
             }
-            uint8_t* data = static_cast<uint8_t*>(pool.data);
             int64_t offset = 0;
             for (int k = 0; k < 2; ++k) {
-                const int64_t size = pool.segment_bytes[k];
-                copy_block(data + to * pool.stride_bytes + offset + e0 * size, data + from * pool.stride_bytes + offset + e0 * size,
-                           (e1 - e0) * size);
+                const int64_t size = pool.segment_bytes[k], at = offset + e0 * size;
+                c.src[k] = static_cast<const uint8_t*>(pool.data) + from * pool.stride_bytes + at;
+                c.dst[k] = static_cast<uint8_t*>(pool.data) + to * pool.stride_bytes + at;
+                c.bytes[k] = static_cast<int>((e1 - e0) * size);
                 offset += pool.entries_per_block * size;
             }
-            break;
+            return c;
         }
+        return c;
+    };
+    for (int64_t unit = blockIdx.x; unit < total[0]; unit += static_cast<int64_t>(kBatch) * gridDim.x) {
+        const int64_t last = total[0] - 1 - unit;
+        const int n = static_cast<int>(min(last / gridDim.x + 1, static_cast<int64_t>(kBatch)));
+        if (tid < n) pieces[tid] = piece_of(static_cast<int>(unit + static_cast<int64_t>(tid) * gridDim.x));
+        __syncthreads();
+        for (int i = 0; i < n; ++i) copy_piece(pieces[i]);
+        __syncthreads();
     }
 }
 
@@ -235,14 +282,20 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
         WUDA_REQUIRE(q.segment_bytes[1] == 0 || static_cast<int64_t>(q.entries_per_block) * q.segment_bytes[0] % 16 == 0,
                      "pool %d: the second segment must start on 16 bytes", i);
         WUDA_REQUIRE(q.stride_bytes >= q.entries_per_block * record, "pool %d: a page does not hold its entries", i);
-        int step = 4;      // entries of a piece: a power of two of them up to kPieceBytes (20 % more where that halves the pieces)
-        while (step * 2 * record <= kPieceBytes * 6 / 5 && step < q.entries_per_block) step *= 2;
-        p.piece_entries[i] = step;
+        int shift = 2;      // entries of a piece: a power of two of them up to kPieceBytes
+        while ((2 * record << shift) <= kPieceBytes && 1 << shift < q.entries_per_block) ++shift;
+        p.piece_shift[i] = shift;
+        p.per_entry[i] = Divisor(q.tokens_per_entry);
+        p.per_block[i] = Divisor(q.entries_per_block);
+        p.per_page[i] = Divisor((q.entries_per_block + (1 << shift) - 1) >> shift);
         // the table's pages bound the pieces of a fork
-        pieces += static_cast<int64_t>(q.table_width) * ((q.entries_per_block + step - 1) / step);
+        pieces += static_cast<int64_t>(q.table_width) * p.per_page[i].by;
     }
     WUDA_REQUIRE(pieces * groups * a.width < INT_MAX, "a reordering of more than 2^31 pieces");
-    for (int i = 0; i < a.num_states; ++i) p.state_pieces += static_cast<int>((a.states[i].row_bytes + kPieceBytes - 1) / kPieceBytes);
+    for (int i = 0; i < a.num_states; ++i) {
+        p.state_pieces += static_cast<int>((a.states[i].row_bytes + kPieceBytes - 1) / kPieceBytes);
+        p.state_first[i + 1] = p.state_pieces;
+    }
     if (groups == 0) return WUDA_OK;
     DeviceInfo dev;
     if (const int st = current_device_info(&dev)) return st;
@@ -252,7 +305,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
         WUDA_CUDA(cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(shared_bytes(kMostRows, kMostSlots))));
     const int64_t most = pieces * rows;
-    const int grid = static_cast<int>(most < 4 * dev.num_sms ? (most > 0 ? most : 1) : 4 * dev.num_sms);
+    const int grid = static_cast<int>(most < kResident * dev.num_sms ? (most > 0 ? most : 1) : kResident * dev.num_sms);
     WUDA_CUDA(launch_pdl(beam_reorder_kernel, dim3(grid), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }

@@ -22,6 +22,7 @@ struct Params {
     const int32_t* new_tokens;
     int rows;
     int32_t* status;
+    Divisor ratio, ring, window, idx_epb, cmp_epb, swa_epb, pieces;
 };
 
 // What is known of a row, in shared memory
@@ -31,16 +32,20 @@ struct Rows {
     int* new_len;
     int* idx_first;   // pages that the rows in front of it take
     int* cmp_first;
+    int* idx_need;    // and that it takes itself
+    int* cmp_need;
     int* start;       // rows + 1
     int* first;       // (load_slots)
     __device__ Rows(int* mem, int rows) {
         slot = mem, old_len = slot + rows, new_len = old_len + rows, idx_first = new_len + rows, cmp_first = idx_first + rows;
-        start = cmp_first + rows, first = start + rows + 1;
+        idx_need = cmp_first + rows, cmp_need = idx_need + rows, start = cmp_need + rows, first = start + rows + 1;
     }
 };
-inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (6ull * rows + 1 + capacity); }
+inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (8ull * rows + 1 + capacity); }
 
-__device__ __forceinline__ int64_t pages_of(int64_t tokens, int ratio, int epb) { return (tokens / ratio + epb - 1) / epb; }
+__device__ __forceinline__ int pages_of(const Params& p, uint32_t tokens, const Divisor& epb) {
+    return static_cast<int>(epb.quotient_up(p.ratio.quotient(tokens)));
+}
 
 __device__ __forceinline__ int cut_count(int count, int capacity, int32_t* status) {
     if (count >= 0 && count <= capacity) return count;
@@ -56,7 +61,12 @@ struct PoolView {
     __device__ int operator()(int page) const { return page < held ? table[page] : free[top - (page - held)]; }
 };
 
-__global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
+// entry `entry` of a request, in page `page` of it, as an entry of the pool
+__device__ __forceinline__ int64_t entry_of(int pool_page, const Divisor& epb, uint32_t page, uint32_t entry) {
+    return static_cast<int64_t>(pool_page) * epb.by + (entry - page * epb.by);
+}
+
+__global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_constant__ Params p) {
     extern __shared__ int mem[];
     __shared__ int scan[3 * 33];
     __shared__ int taken[2];
@@ -84,8 +94,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
         if (slot < 0) continue;
         const int old = a.lengths[slot];
         const int64_t now = static_cast<int64_t>(old) + n;
-        const int64_t idx_pages = pages_of(now, a.ratio, a.idx_entries_per_block), cmp_pages = pages_of(now, a.ratio, a.cmp_entries_per_block);
-        if (old < 0 || n < 0 || now > INT_MAX || idx_pages > a.table_width || cmp_pages > a.table_width) {
+        const bool counts = old >= 0 && n >= 0 && now <= INT_MAX;
+        const int idx_pages = counts ? pages_of(p, static_cast<uint32_t>(now), p.idx_epb) : 0;
+        const int cmp_pages = counts ? pages_of(p, static_cast<uint32_t>(now), p.cmp_epb) : 0;
+        if (!counts || idx_pages > a.table_width || cmp_pages > a.table_width) {
             report(status, WUDA_DEV_BAD_LENGTH);
             r.slot[b] = -1;
             continue;
@@ -94,8 +106,8 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
         r.new_len[b] = static_cast<int>(now);
         r.idx_first[b] = sum[1];
         r.cmp_first[b] = sum[2];
-        sum[1] += static_cast<int>(idx_pages - pages_of(old, a.ratio, a.idx_entries_per_block));
-        sum[2] += static_cast<int>(cmp_pages - pages_of(old, a.ratio, a.cmp_entries_per_block));
+        sum[1] += r.idx_need[b] = idx_pages - pages_of(p, old, p.idx_epb);
+        sum[2] += r.cmp_need[b] = cmp_pages - pages_of(p, old, p.cmp_epb);
     }
     block_exclusive_sum<3, kThreads>(sum, total, scan);
     if (tid == 0) {
@@ -110,10 +122,8 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
         const int begin = r.start[b] + sum[0];
         r.start[b] = min(begin, a.max_tokens);
         if (r.slot[b] < 0) continue;
-        const int64_t old = r.old_len[b], now = r.new_len[b];
         const int idx_first = r.idx_first[b] + sum[1], cmp_first = r.cmp_first[b] + sum[2];
-        const int idx_need = static_cast<int>(pages_of(now, a.ratio, a.idx_entries_per_block) - pages_of(old, a.ratio, a.idx_entries_per_block));
-        const int cmp_need = static_cast<int>(pages_of(now, a.ratio, a.cmp_entries_per_block) - pages_of(old, a.ratio, a.cmp_entries_per_block));
+        const int idx_need = r.idx_need[b], cmp_need = r.cmp_need[b];
         if (begin + static_cast<int64_t>(n) > a.max_tokens) {
             report(status, WUDA_DEV_BAD_LENGTH);
             r.slot[b] = -1;
@@ -157,13 +167,13 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
     // ---- the outputs, a task per warp: 256 columns of one pool's block table, a row's values and window entries, or 32 tokens
     const int window_pages = (a.window + a.swa_entries_per_block - 1) / a.swa_entries_per_block;
     const int tokens = r.start[rows];
-    const int pieces = (a.table_width + kPiece - 1) / kPiece, tables = rows * 2 * pieces;
+    const int pieces = static_cast<int>(p.pieces.by), tables = rows * 2 * pieces;
     const int tasks = tables + rows + (tokens + 31) / 32;
     for (int task = blockIdx.x * kWarps + warp; task < tasks; task += gridDim.x * kWarps) {
         if (task < tables) {
-            const int piece = task % pieces, of = task / pieces, b = of >> 1;
+            const int of = static_cast<int>(p.pieces.quotient(task)), piece = task - of * pieces, b = of >> 1;
             const bool cmp = of & 1;
-            const int epb = cmp ? a.cmp_entries_per_block : a.idx_entries_per_block;
+            const Divisor epb = cmp ? p.cmp_epb : p.idx_epb;
             const int slot = r.slot[b];
             int32_t* out = (cmp ? a.cmp_block_table : a.idx_block_table) + b * a.block_table_stride;
             PoolView pool = {};
@@ -171,8 +181,8 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
             int32_t* table = nullptr;
             if (slot >= 0) {
                 table = (cmp ? a.cmp_table : a.idx_table) + slot * a.table_stride;
-                pages = static_cast<int>(pages_of(r.new_len[b], a.ratio, epb));
-                pool = {table, cmp ? a.cmp_free : a.idx_free, static_cast<int>(pages_of(r.old_len[b], a.ratio, epb)),
+                pages = pages_of(p, r.new_len[b], epb);
+                pool = {table, cmp ? a.cmp_free : a.idx_free, pages - (cmp ? r.cmp_need[b] : r.idx_need[b]),
                         cmp ? r.cmp_first[b] : r.idx_first[b]};
             }
             int page[kPiece / 32];
@@ -193,12 +203,11 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
             const int valid = min(now, a.window);
             const int32_t* pages = a.swa_table + static_cast<int64_t>(max(slot, 0)) * window_pages;
             for (int i = lane; i < a.window; i += 32) {
-                const int ring = i < valid ? (now - valid + i) % a.window : 0;
-                a.swa_indices[static_cast<int64_t>(b) * a.window + i] =
-                    i < valid ? pages[ring / a.swa_entries_per_block] * a.swa_entries_per_block + ring % a.swa_entries_per_block : -1;
+                const uint32_t ring = i < valid ? p.window.rest(now - valid + i) : 0, page = p.swa_epb.quotient(ring);
+                a.swa_indices[static_cast<int64_t>(b) * a.window + i] = i < valid ? static_cast<int>((pages[page] - page) * p.swa_epb.by + ring) : -1;
             }
             if (lane == 0) {
-                const int entries = now / a.ratio;
+                const int entries = static_cast<int>(p.ratio.quotient(now));
                 a.n_compressed[b] = entries;
                 a.cmp_lengths[b] = min(entries, a.topk);
                 a.swa_lengths[b] = valid;
@@ -216,20 +225,18 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const Params p) {
             if (slot >= 0) {
                 const int old = r.old_len[b], now = r.new_len[b];
                 pos = old + t - r.start[b];
-                if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + pos % a.ring_entries;
+                if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + p.ring.rest(pos);
                 if (pos >= now - a.window) {
-                    const int ring = pos % a.window;
-                    swa = static_cast<int64_t>(a.swa_table[static_cast<int64_t>(slot) * window_pages + ring / a.swa_entries_per_block]) *
-                              a.swa_entries_per_block + ring % a.swa_entries_per_block;
+                    const uint32_t ring = p.window.rest(pos), page = p.swa_epb.quotient(ring);
+                    swa = entry_of(a.swa_table[static_cast<int64_t>(slot) * window_pages + page], p.swa_epb, page, ring);
                 }
-                if ((pos + 1u) % a.ratio == 0) {
-                    const int entry = static_cast<int>((pos + 1u) / a.ratio) - 1;
-                    const PoolView ip = {a.idx_table + slot * a.table_stride, a.idx_free,
-                                         static_cast<int>(pages_of(old, a.ratio, a.idx_entries_per_block)), r.idx_first[b]};
-                    const PoolView cp = {a.cmp_table + slot * a.table_stride, a.cmp_free,
-                                         static_cast<int>(pages_of(old, a.ratio, a.cmp_entries_per_block)), r.cmp_first[b]};
-                    idx = static_cast<int64_t>(ip(entry / a.idx_entries_per_block)) * a.idx_entries_per_block + entry % a.idx_entries_per_block;
-                    cmp = static_cast<int64_t>(cp(entry / a.cmp_entries_per_block)) * a.cmp_entries_per_block + entry % a.cmp_entries_per_block;
+                const uint32_t done = p.ratio.quotient(pos + 1u);
+                if (done * p.ratio.by == pos + 1u) {
+                    const uint32_t entry = done - 1, idx_page = p.idx_epb.quotient(entry), cmp_page = p.cmp_epb.quotient(entry);
+                    const PoolView ip = {a.idx_table + slot * a.table_stride, a.idx_free, pages_of(p, old, p.idx_epb), r.idx_first[b]};
+                    const PoolView cp = {a.cmp_table + slot * a.table_stride, a.cmp_free, pages_of(p, old, p.cmp_epb), r.cmp_first[b]};
+                    idx = entry_of(ip(idx_page), p.idx_epb, idx_page, entry);
+                    cmp = entry_of(cp(cmp_page), p.cmp_epb, cmp_page, entry);
                 }
             }
             a.pos[t] = pos;
@@ -280,6 +287,9 @@ extern "C" int wuda_step_tables(const wuda_step_tables_args* args, const int32_t
         WUDA_CUDA(cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(shared_bytes(kMostRows, kMostSlots))));
     Params p = {a, slots, new_tokens, rows, status_word};
+    p.ratio = Divisor(a.ratio), p.ring = Divisor(a.ring_entries), p.window = Divisor(a.window);
+    p.idx_epb = Divisor(a.idx_entries_per_block), p.cmp_epb = Divisor(a.cmp_entries_per_block), p.swa_epb = Divisor(a.swa_entries_per_block);
+    p.pieces = Divisor((a.table_width + kPiece - 1) / kPiece);
     const int64_t tokens = new_tokens ? a.max_tokens : rows;
     const int64_t tasks = static_cast<int64_t>(rows) * (2 * ((a.table_width + kPiece - 1) / kPiece) + 1) + (tokens + 31) / 32;
     const int grid = static_cast<int>(tasks < static_cast<int64_t>(dev.num_sms) * kWarps ? (tasks + kWarps - 1) / kWarps : dev.num_sms);
