@@ -1,8 +1,8 @@
 // Beam reordering: slots of the new beams, and the copies of what forks take over from their parents.
 //
-// Of a group's W <= 32 beams lane j of a warp looks at new beam j: match_any finds the children of one parent (the lowest keeps the
-// parent's slot), one OR over the lanes the parents that have a child; the other beams' slots go to the further children in order.
-// Sources (parents) and destinations (beams without a child) are different slots, so all copies run at the same time and in place.
+// A lane looks at one new beam: match_any finds the children of one parent, of which the first keeps the parent's slot; one OR over the
+// lanes gives the parents that have a child, and the slots of the other beams go to the further children in order.  Sources (parents)
+// and destinations (beams without a child) are different slots, so all copies run at the same time and in place.
 //
 // Every CTA works out all groups for itself in shared memory, with the number of pieces that each fork's copy has (a few KB
 // each: rows of the states, entries of one page of a pool); a scan over the forks numbers the pieces and the CTAs take them in turn.
@@ -27,11 +27,12 @@ struct Params {
     int state_first[WUDA_BEAM_MAX_STATES + 1];   // the first piece of each state's rows, the pieces of all
     int state_pieces;
     int piece_shift[WUDA_BEAM_MAX_POOLS];        // entries of a page that are copied at a time: 2 ^ this, at least 4
+    Divisor per_group;                           // beams
     Divisor per_entry[WUDA_BEAM_MAX_POOLS], per_block[WUDA_BEAM_MAX_POOLS], per_page[WUDA_BEAM_MAX_POOLS];      // tokens, entries, pieces
     int32_t* status;
 };
 
-inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (6ull * rows + 1 + capacity); }
+inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (8ull * rows + capacity); }
 
 __device__ __forceinline__ int lowest_but(uint32_t set, int n) {      // the n-th lowest member, -1 where there are fewer
     for (; n > 0 && set; --n) set &= set - 1;
@@ -94,19 +95,21 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
     const wuda_beam_reorder_args& a = p.a;
     const int width = a.width, rows = p.groups * width, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int* slot = mem;                 // of the beams now
-    int* source = slot + rows;       // of new beam j: the beam of its group that it continues; then the slot that its own is filled from, -1 no fork
-    int* own = source + rows;        // of new beam j: its slot
-    int* begin = own + rows;         // of new beam j: the number of its first piece
-    int* length = begin + rows + 1;  // of the beams now; then of what a fork copies
-    int* common = length + rows;     // their shared lengths
-    int* first = common + rows;      // (load_slots)
+    int* length = slot + rows;       // ... their tokens
+    int* common = length + rows;     // ... and shared tokens
+    int* parents = common + rows;    // of new beam j: the beam of its group that it continues
+    int* source = parents + rows;    // the slot that its own is filled from, -1: no fork
+    int* donor = source + rows;      // ... and the beam that has it
+    int* own = donor + rows;         // its slot
+    int* begin = own + rows;         // the number of its first piece
+    int* first = begin + rows;       // (load_slots)
     int32_t* status = blockIdx.x == 0 ? p.status : nullptr;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int per = (rows + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, rows), b1 = min(b0 + per, rows);
     for (int b = b0; b < b1; ++b) {
-        source[b] = p.parents[b];
+        parents[b] = p.parents[b];
         const int s = p.slots[b];
         const bool inside = s >= 0 && s < a.capacity;
         length[b] = inside ? a.lengths[s] : -1;
@@ -115,65 +118,57 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
     load_slots(p.slots, b0, b1, a.capacity, slot, first, status);
     __syncthreads();
 
-    // ---- new slots and forks, a group per warp
-    for (int g = warp; g < p.groups; g += kWarps) {
-        const int at = g * width + lane;
-        const bool mine = lane < width;
-        const int now = mine ? slot[at] : -1, tokens = mine ? length[at] : -1, shared = mine ? common[at] : 0;
-        int parent = mine ? source[at] : -1;
-        if (parent < -1 || parent >= width) {
-            report(status, WUDA_DEV_BAD_PARENT);
-            parent = -1;
+    // ---- new slots and forks, and how much each fork copies: a lane per new beam, as many whole groups to a warp as fit
+    const int together = static_cast<int>(p.per_group.quotient(32)), in_warp = static_cast<int>(p.per_group.quotient(lane));
+    for (int g0 = warp * together; g0 < p.groups; g0 += kWarps * together) {
+        const int at = (g0 + in_warp) * width, base = in_warp * width, j = lane - base, b = at + j;
+        const bool mine = in_warp < together && g0 + in_warp < p.groups;
+        const uint32_t below = (1u << lane) - 1, group = mine ? (width < 32 ? (1u << width) - 1 : 0xffffffffu) << base : 0;
+        int parent = mine ? parents[b] : -1;
+        const bool live = mine && slot[b] >= 0;
+        const uint32_t all_live = __ballot_sync(0xffffffffu, live);
+        if (parent < -1 || parent >= width) report(status, WUDA_DEV_BAD_PARENT);
+        if (parent < 0 || parent >= width || !(all_live >> (base + parent) & 1)) parent = -1;
+        const uint32_t siblings = __match_any_sync(0xffffffffu, parent >= 0 ? base + parent : -1);
+        const bool keeps = parent >= 0 && lane == __ffs(siblings) - 1;
+        const uint32_t has_child = __reduce_or_sync(0xffffffffu, parent >= 0 ? 1u << (base + parent) : 0u);
+        const uint32_t further = __ballot_sync(0xffffffffu, parent >= 0 && !keeps) & group;
+        const uint32_t orphans = __ballot_sync(0xffffffffu, mine && parent < 0) & group;
+        if (!mine) continue;
+        // (there are at least as many places as further children, unless slots were refused)
+        const uint32_t places = (all_live & ~has_child & group) >> base;
+        const int place = keeps ? parent : lowest_but(places, parent >= 0 ? __popc(further & below) : __popc(further) + __popc(orphans & below));
+        int to = place >= 0 ? slot[at + place] : -1, from = -1, pieces = 0;
+        if (parent >= 0 && !keeps && to >= 0) {
+            const int tokens = length[at + parent], shared = common[at + parent];
+            bool good = tokens >= 0 && shared >= 0 && length[at + place] == tokens && common[at + place] == shared;
+            if (good) {
+                from = slot[at + parent];
+                pieces = p.state_pieces;
+#pragma unroll
+                for (int i = 0; i < WUDA_BEAM_MAX_POOLS; ++i) {
+                    if (i >= a.num_pools) break;
+                    const Span s = span_of(p, i, tokens, shared);
+                    good = good && s.pages <= a.pools[i].table_width;
+                    if (good) pieces += pieces_of(p, i, s);
+                }
+            }
+            if (!good) {
+                report(status, WUDA_DEV_BAD_LENGTH);
+                to = from = -1;
+                pieces = 0;
+            }
         }
-        const int from = __shfl_sync(0xffffffffu, now, max(parent, 0));
-        if (parent >= 0 && from < 0) parent = -1;
-        const uint32_t children = __match_any_sync(0xffffffffu, parent);
-        const bool keeps = parent >= 0 && lane == __ffs(children) - 1;
-        const uint32_t has_child = __reduce_or_sync(0xffffffffu, parent >= 0 ? 1u << parent : 0u);
-        const uint32_t places = __ballot_sync(0xffffffffu, now >= 0) & ~has_child;
-        const uint32_t further = __ballot_sync(0xffffffffu, parent >= 0 && !keeps);
-        const uint32_t orphans = __ballot_sync(0xffffffffu, mine && parent < 0);
-        const uint32_t below = (1u << lane) - 1;
-        // (a parent's further children are at most as many as there are places, unless slots were refused)
-        const int place = keeps ? parent : (parent >= 0 ? lowest_but(places, __popc(further & below))
-                                                        : lowest_but(places, __popc(further) + __popc(orphans & below)));
-        int to = __shfl_sync(0xffffffffu, now, max(place, 0));
-        const int to_tokens = __shfl_sync(0xffffffffu, tokens, max(place, 0)), to_shared = __shfl_sync(0xffffffffu, shared, max(place, 0));
-        const int from_tokens = __shfl_sync(0xffffffffu, tokens, max(parent, 0)), from_shared = __shfl_sync(0xffffffffu, shared, max(parent, 0));
-        if (place < 0) to = -1;
-        bool fork = parent >= 0 && !keeps && to >= 0;
-        if (fork && (from_tokens < 0 || from_shared < 0 || to_tokens != from_tokens || to_shared != from_shared)) {
-            report(status, WUDA_DEV_BAD_LENGTH);
-            fork = false;
-            to = -1;
-        }
-        __syncwarp();
-        if (mine) {
-            source[at] = fork ? from : -1;
-            own[at] = to;
-            length[at] = from_tokens;
-            common[at] = from_shared;
-        }
+        source[b] = from;
+        own[b] = to;
+        donor[b] = from >= 0 ? at + parent : 0;
+        begin[b] = pieces;
     }
     __syncthreads();
-
-    // ---- how much each fork copies
     int sum[1] = {0}, total[1];
     for (int b = b0; b < b1; ++b) {
+        const int pieces = begin[b];
         begin[b] = sum[0];
-        if (source[b] < 0) continue;
-        bool good = true;
-        int pieces = p.state_pieces;
-        for (int i = 0; i < a.num_pools; ++i) {
-            const Span s = span_of(p, i, length[b], common[b]);
-            good = good && s.pages <= a.pools[i].table_width;
-            if (good) pieces += pieces_of(p, i, s);
-        }
-        if (!good) {
-            report(status, WUDA_DEV_BAD_LENGTH);
-            source[b] = own[b] = -1;
-            continue;
-        }
         sum[0] += pieces;
     }
     block_exclusive_sum<1, kThreads>(sum, total, scan);
@@ -192,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
             if (begin[mid] <= unit) b = mid, lo = mid + 1;
             else hi = mid;
         }
-        const int src = source[b], dst = own[b];
+        const int src = source[b], dst = own[b], tokens = length[donor[b]], shared = common[donor[b]];
         int piece = unit - begin[b];
         if (piece < p.state_pieces) {
             int i = 0;
@@ -204,9 +199,11 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
             return c;
         }
         piece -= p.state_pieces;
-        for (int i = 0; i < a.num_pools; ++i) {
+#pragma unroll
+        for (int i = 0; i < WUDA_BEAM_MAX_POOLS; ++i) {
+            if (i >= a.num_pools) break;
             const wuda_beam_pool& pool = a.pools[i];
-            const Span s = span_of(p, i, length[b], common[b]);
+            const Span s = span_of(p, i, tokens, shared);
             const int n = pieces_of(p, i, s);
             if (piece >= n) {
                 piece -= n;
@@ -222,6 +219,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
                 return c;
             }
             int64_t offset = 0;
+#pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int64_t size = pool.segment_bytes[k], at = offset + e0 * size;
                 c.src[k] = static_cast<const uint8_t*>(pool.data) + from * pool.stride_bytes + at;
@@ -263,6 +261,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
     WUDA_REQUIRE(groups == 0 || (slots_out != slots && slots_out != parents), "slots_out must be an array of its own");
     Params p = {};
     p.a = a;
+    p.per_group = Divisor(a.width);
     p.parents = parents, p.slots = slots, p.slots_out = slots_out, p.groups = groups, p.status = status_word;
     int64_t pieces = 0;
     for (int i = 0; i < a.num_states; ++i) {
