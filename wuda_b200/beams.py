@@ -12,6 +12,7 @@ from typing import Tuple
 import torch
 
 from . import _lib
+from . import ops as _ops
 from ._lib import check, lib
 from .ops import _on_current_device, _require, _stream
 
@@ -65,7 +66,7 @@ class BeamReorder:
         self.lengths, self.shared_lengths, self.states, self.pools = lengths, shared_lengths, list(states), list(pools)
         self.width, self.status_word = int(width), status_word
         self._device, self._args = dev.index, a
-        self._args_ref = ctypes.byref(a)
+        self._args_ref, self._address = ctypes.byref(a), ctypes.addressof(a)
         self._status = None if status_word is None else status_word.data_ptr()
         check(lib.wuda_beam_reorder(self._args_ref, None, None, None, 0, None, None))
 
@@ -74,6 +75,8 @@ class BeamReorder:
         beams' request slots (-1: none).  Fills and returns slots_out int32 [groups, width], a tensor of its own: the first child
         of a beam keeps its slot, the others take the slots of beams without children, with a copy of their parent's contents.
         Lengths and page tables stay as they are (the slots of a group hold equally many tokens)."""
+        if _ops._fast.beam_reorder(self._address, parents, slots, slots_out, self.width, self._device, self._status):
+            return slots_out
         groups = parents.numel() // self.width
         for t, name in ((parents, "parents"), (slots, "slots"), (slots_out, "slots_out")):
             if not (t.dtype is torch.int32 and t.is_contiguous() and t.numel() == groups * self.width and t.is_cuda and

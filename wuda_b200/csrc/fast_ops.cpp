@@ -33,7 +33,8 @@ using at::Tensor;
     X(wuda_mqa_logits_fp8) X(wuda_mqa_logits_fp4) X(wuda_topk) X(wuda_rmsnorm_quant_fp8) X(wuda_rope_quant_fp8)       \
     X(wuda_gemm_fp8_scratch_bytes) X(wuda_gemm_bf16_scratch_bytes) X(wuda_gemm_nvfp4_scratch_bytes)                   \
     X(wuda_gemm_fp8_blockscaled) X(wuda_gemm_fp8_blockscaled_pow2) X(wuda_gemm_fp8_fp4_pow2) X(wuda_gemm_bf16)        \
-    X(wuda_gemm_nvfp4) X(wuda_sparse_mla_workspace_bytes) X(wuda_sparse_mla_decode)
+    X(wuda_gemm_nvfp4) X(wuda_sparse_mla_workspace_bytes) X(wuda_sparse_mla_decode)                                   \
+    X(wuda_step_tables) X(wuda_beam_select_workspace_bytes) X(wuda_beam_select) X(wuda_beam_reorder)
 
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -433,6 +434,97 @@ PyObject* sparse_mla_decode(PyObject* const* p) {
     return result(p[9], made);
 }
 
+// ---------------------------------------------------------------- between two steps
+void need_current(const Tensor& t) { need(t.get_device() == c10::cuda::current_device()); }
+
+// A plan's argument struct, whose owner is the caller.
+template <typename T>
+const T* plan(PyObject* address) {
+    need(PyLong_CheckExact(address));
+    const void* p = PyLong_AsVoidPtr(address);
+    need(p != nullptr);
+    return static_cast<const T*>(p);
+}
+int32_t* status_address(PyObject* o) {
+    if (o == Py_None) return nullptr;
+    need(PyLong_CheckExact(o));
+    return static_cast<int32_t*>(PyLong_AsVoidPtr(o));
+}
+
+// address of the arguments, slots, new_tokens, max_rows, device, address of the status word
+PyObject* step_tables(PyObject* const* p) {
+    const auto* args = plan<wuda_step_tables_args>(p[0]);
+    const Tensor& slots = dense(p[1], ScalarType::Int);
+    need(slots.numel() <= integer(p[3]) && slots.get_device() == integer(p[4]));
+    need_current(slots);
+    const int32_t* tokens = nullptr;
+    if (p[2] != Py_None) {
+        const Tensor& t = dense(p[2], ScalarType::Int);
+        need(t.numel() == slots.numel() && t.get_device() == slots.get_device());
+        tokens = static_cast<const int32_t*>(t.data_ptr());
+    }
+    call(entries.wuda_step_tables, args, static_cast<const int32_t*>(slots.data_ptr()), tokens, int32(slots.numel()), status_address(p[5]),
+         current_stream());
+    Py_RETURN_TRUE;
+}
+
+// address of the arguments, parents, slots, slots_out, width, device, address of the status word
+PyObject* beam_reorder(PyObject* const* p) {
+    const auto* args = plan<wuda_beam_reorder_args>(p[0]);
+    const Tensor& parents = dense(p[1], ScalarType::Int);
+    const Tensor& slots = dense(p[2], ScalarType::Int);
+    const Tensor& out = dense(p[3], ScalarType::Int);
+    const int64_t width = integer(p[4]), n = parents.numel();
+    need(width >= 1 && n % width == 0 && slots.numel() == n && out.numel() == n && parents.get_device() == integer(p[5]) &&
+         slots.get_device() == parents.get_device() && out.get_device() == parents.get_device());
+    need_current(parents);
+    call(entries.wuda_beam_reorder, args, static_cast<const int32_t*>(parents.data_ptr()), static_cast<const int32_t*>(slots.data_ptr()),
+         static_cast<int32_t*>(out.data_ptr()), int32(n / width), status_address(p[6]), current_stream());
+    Py_RETURN_TRUE;
+}
+
+// logits, scores, k, finished, eos_token, streams, the bytes of counters in front of a scratch
+PyObject* beam_select(PyObject* const* p) {
+    const Tensor& logits = cuda_tensor(p[0]);
+    const Tensor& scores = dense(p[1], ScalarType::Float);
+    const ScalarType type = logits.scalar_type();
+    need(logits.dim() == 3 && (type == ScalarType::BFloat16 || type == ScalarType::Half || type == ScalarType::Float) &&
+         (logits.stride(2) == 1 || logits.size(2) == 1));
+    need_current(logits);
+    wuda_beam_select_args a = {};
+    a.groups = int32(logits.size(0)), a.width = int32(logits.size(1)), a.vocab = int32(logits.size(2));
+    need(scores.dim() == 2 && scores.size(0) == a.groups && scores.size(1) == a.width && scores.get_device() == logits.get_device() && a.groups > 0);
+    a.k = p[2] == Py_None ? a.width : int32(integer(p[2]));
+    a.eos_token = -1;
+    if (p[4] != Py_None) {
+        a.eos_token = int32(integer(p[4]));
+        need(a.eos_token >= 0);      // (-1 is the library's own word for none)
+    }
+    if (p[3] != Py_None) {
+        const Tensor& finished = dense(p[3], ScalarType::Bool);
+        need(finished.dim() == 2 && finished.size(0) == a.groups && finished.size(1) == a.width && finished.get_device() == logits.get_device());
+        a.finished = static_cast<const uint8_t*>(finished.data_ptr());
+    }
+    a.logits_type = type == ScalarType::BFloat16 ? 0 : type == ScalarType::Half ? 1 : 2;
+    a.logits = logits.data_ptr(), a.group_stride = logits.stride(0), a.beam_stride = logits.stride(1);
+    a.scores = static_cast<const float*>(scores.data_ptr());
+    void* stream = current_stream();
+    const int64_t wanted = entries.wuda_beam_select_workspace_bytes(a.groups, a.width, a.vocab, a.k, a.logits_type), front = integer(p[6]);
+    need(wanted >= 0);
+    const Scratch scratch(p[5], logits, stream, wanted + front);
+    a.counters = static_cast<int32_t*>(scratch.at);
+    a.workspace = static_cast<char*>(scratch.at) + front, a.workspace_bytes = scratch.bytes - front;
+    const Tensor out[4] = {fresh({a.groups, a.k}, ScalarType::Float, logits), fresh({a.groups, a.k}, ScalarType::Int, logits),
+                           fresh({a.groups, a.k}, ScalarType::Int, logits), fresh({a.groups, a.k}, ScalarType::Bool, logits)};
+    a.scores_out = static_cast<float*>(out[0].data_ptr()), a.parents_out = static_cast<int32_t*>(out[1].data_ptr());
+    a.tokens_out = static_cast<int32_t*>(out[2].data_ptr()), a.finished_out = static_cast<uint8_t*>(out[3].data_ptr());
+    call(entries.wuda_beam_select, static_cast<const wuda_beam_select_args*>(&a), stream);
+    PyObject* result = PyTuple_New(4);
+    need(result != nullptr);
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(out[i]));
+    return result;
+}
+
 // ---------------------------------------------------------------- module
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -474,6 +566,9 @@ PyMethodDef methods[] = {{"bind", bind, METH_O, nullptr},
                          WUDA_METHOD("bf16_gemm", bf16_gemm, 6),
                          WUDA_METHOD("nvfp4_gemm", nvfp4_gemm, 9),
                          WUDA_METHOD("sparse_mla_decode", sparse_mla_decode, 13),
+                         WUDA_METHOD("step_tables", step_tables, 6),
+                         WUDA_METHOD("beam_reorder", beam_reorder, 7),
+                         WUDA_METHOD("beam_select", beam_select, 7),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -234,6 +234,9 @@ def beam_select(logits, scores, k=None, *, finished=None, eos_token=None):
     beam whose score is not finite has no continuation, a finished beam (finished bool [groups, width], with an
     eos_token) only itself with eos_token; the logits of both are not read.  Where fewer than k continuations are left, the rest is
     (-inf, -1, -1, False).  groups <= 256, width <= 32, k <= 64."""
+    done = _fast.beam_select(logits, scores, k, finished, eos_token, _beam_scratch._streams, FLAG_BYTES)
+    if done is not None:
+        return done
     _require(logits.dim() == 3 and logits.dtype in _LOGITS_TYPES and _on_current_device(logits) and
              (logits.stride(2) == 1 or logits.size(2) == 1),
              "logits must be bf16, fp16 or fp32 [groups, width, vocab] on the current CUDA device with unit inner stride")
@@ -244,6 +247,7 @@ def beam_select(logits, scores, k=None, *, finished=None, eos_token=None):
         _require(finished.device == logits.device and finished.dtype == torch.bool and finished.is_contiguous() and
                  tuple(finished.shape) == (groups, width), "finished must be contiguous bool [groups, width] on the logits' device")
         _require(eos_token is not None, "finished beams need an eos_token")
+    _require(eos_token is None or 0 <= eos_token < vocab, "eos_token must be a token of the vocabulary")
     k = width if k is None else int(k)
     need = lib.wuda_beam_select_workspace_bytes(groups, width, vocab, k, _LOGITS_TYPES[logits.dtype])
     _require(need >= 0, "beam_select: groups <= 256, width in [1, 32], vocab in [1, 2^24] and k in [1, 64] are implemented")

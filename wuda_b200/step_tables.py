@@ -13,6 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
+from . import ops as _ops
 from .kv_cache import M1_BODY, RATIO, WIN
 from .ops import _on_current_device, _require, _stream
 
@@ -95,7 +96,7 @@ class StepTables:
             idx_entries_per_block=idx_entries_per_block, cmp_entries_per_block=cmp_entries_per_block,
             swa_entries_per_block=swa_entries_per_block, ratio=ratio, ring_entries=ring_entries, window=window, topk=topk,
             **{name: p(t) for name, t in self.out.items()})
-        self._args_ref = ctypes.byref(self._args)
+        self._args_ref, self._address = ctypes.byref(self._args), ctypes.addressof(self._args)
         self._status = None if status_word is None else status_word.data_ptr()
         check(lib.wuda_step_tables(self._args_ref, None, None, 0, None, None))
 
@@ -108,6 +109,8 @@ class StepTables:
         What lies behind the last token and the last row is left as it was.  A row that cannot be served (a slot given twice,
         no free page, a context beyond the tables) is reported in status_word and left out: positions 0, destinations -1,
         lengths 0; its state stays."""
+        if _ops._fast.step_tables(self._address, slots, new_tokens, self.max_rows, self._device, self._status):
+            return self.out
         rows = slots.numel()
         if not (slots.dtype is torch.int32 and slots.is_contiguous() and rows <= self.max_rows and slots.is_cuda and
                 slots.get_device() == self._device == torch._C._cuda_getDevice()):
