@@ -13,8 +13,8 @@
 // thread gets depends on the element's number alone, not on the row's alignment, so equal rows have equal sums.
 //
 // Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's k-th largest
-// logit, raised in front of the tiles 0, 3, 15, ..; a vector of loads that passes it (a handful per tile) is noted and looked at in the
-// end, with the last bound.  No barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
+// logit, raised in front of the tiles 0, 3, 15, ..; what a thread has of a tile in which it sees a logit beyond the bound is noted (a
+// handful per tile) and looked at in the end, with the last bound.  No barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
 // The CTA that completes a group's counter merges its lists: the k-th largest of the lists' first candidates bounds what can be among
 // the k best, and the few that pass are ranked by counting.
@@ -33,8 +33,8 @@ namespace beams {
 
 constexpr int kVectors = 4;                 // 16-byte loads per thread and tile
 constexpr int kMostK = 64, kMostWidth = 32, kMostGroups = 256;
-constexpr int kList = 1024;                 // candidates that a chunk's CTA holds, and vectors with candidates that it notes
-constexpr int kNotes = 384;                 // ... of which it keeps the contents
+constexpr int kList = 1024;                 // candidates that a chunk's CTA holds
+constexpr int kNotesOfBlock = 160, kNotesAllOfBlock = 1024; // notes of a CTA's warps with their contents, and without
 constexpr int kEntries = 2048;              // candidates of all chunks of a group
 constexpr int kMostChunks = 64;
 constexpr int kMostLists = 256;             // of a group
@@ -195,10 +195,11 @@ __device__ __forceinline__ double unordered(Key u) { return __longlong_as_double
 // The work of a CTA of kThreads threads
 template <int kThreads>
 struct Block {
-static constexpr int kWarps = kThreads / 32;
+static constexpr int kWarps = kThreads / 32, kNotes = kNotesOfBlock / kWarps, kNotesAll = kNotesAllOfBlock / kWarps;
 
 struct Shared {
-    int count, vectors;                     // candidates, and vectors that may hold some (those beyond kList are lost)
+    int count;                              // candidates (those beyond kList are lost)
+    bool lost;                              // more was to be noted than there are places for
     float bound;                            // the k-th largest logit so far, or less
     int hits[3];
     float warp_ref[kWarps];
@@ -207,9 +208,9 @@ struct Shared {
     union {
         struct {                            // a chunk
             alignas(16) Key list[kList];
-            alignas(16) uint4 note[kNotes];
+            alignas(16) uint4 note[kWarps][kNotes][kVectors];      // what a thread had of a tile in which a logit passed the bound
             alignas(16) float part_max[128];           // maxima of parts of the tiles
-            int vector[kList];                         // vectors with a logit beyond the bound of their tile
+            int noted[kWarps][kNotesAll];              // ... whose: tile * threads + thread
         };
         struct {                            // a group's lists
             alignas(16) Key entry[kEntries];
@@ -365,7 +366,8 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
     const int c0 = number * p.chunk_vectors * kVec, end = min(a.vocab, c0 + p.chunk_vectors * kVec);
     if (tid == 0) {
-        sh.count = sh.vectors = 0;
+        sh.count = 0;
+        sh.lost = false;
         sh.bound = -INFINITY;
     }
     constexpr int kTile = kThreads * kVectors * kVec;
@@ -386,6 +388,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     if (!(fabsf(a.scores[row_number]) < INFINITY)) return;
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    int noted = 0;        // of the warp's vectors
     int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, ..
     for (int tile = 0; tile < tiles; ++tile) {
         uint32_t w[4 * kVectors];
@@ -395,15 +398,15 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
             w[4 * u + 2] = without_nan<T>(next[u].z), w[4 * u + 3] = without_nan<T>(next[u].w);
         }
         if (tile + 1 < tiles) fetch(tile + 1);
-        // ---- the maximum of some of the words
-        const auto maximum = [&](int from, int n) {
-            uint32_t m = w[from];
+        // ---- the maximum
+        const auto maximum = [&] {
+            uint32_t m = w[0];
 #pragma unroll
-            for (int i = 1; i < n; ++i) m = max_words<T>(m, w[from + i]);
+            for (int i = 1; i < 4 * kVectors; ++i) m = max_words<T>(m, w[i]);
             const float2 f = pair_of<T>(m);
             return fmaxf(f.x, f.y);
         };
-        float top = maximum(0, 4 * kVectors);
+        float top = maximum();
         if (top == INFINITY) {
 #pragma unroll
             for (int i = 0; i < 4 * kVectors; ++i) {
@@ -415,7 +418,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
                     if (f.y == INFINITY) w[i] = (w[i] & 0xffffu) | (Type<T>::kMasked & 0xffff0000u);
                 }
             }
-            top = maximum(0, 4 * kVectors);
+            top = maximum();
         }
         // ---- sum of exp(x - ref)
         if (top - ref > kGrow) {
@@ -441,39 +444,40 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
             refresh = 4 * refresh + 3;
             bound = raise_bound(sh, so_far, k, bound, &with_equal);
         }
-        if (with_equal ? top >= bound : top > bound) {
+        const bool hit = with_equal ? top >= bound : top > bound;
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+        if (hits) {      // places without atomics: each warp has a list of its own
+            const int at = noted + __popc(hits & ((1u << lane) - 1));
+            if (hit && at < kNotesAll) sh.noted[warp][at] = tile * kThreads + tid;
+            if (hit && at < kNotes) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u) {
-                const float high = maximum(4 * u, 4);
-                if (with_equal ? high >= bound : high > bound) {
-                    const int at = atomicAdd(&sh.vectors, 1);
-                    if (at < kList) sh.vector[at] = (tile * kVectors + u) * kThreads + tid;
-                    if (at < kNotes) sh.note[at] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
-                }
+                for (int u = 0; u < kVectors; ++u) sh.note[warp][at][u] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
             }
+            noted += __popc(hits);
         }
     }
 
-    // ---- candidates: the elements of the noted vectors that pass the last bound
+    // ---- candidates: the noted elements that pass the last bound
     bool raised;
     if (4 * (tiles - 1) + 3 != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
     else __syncthreads();      // (it was raised with the last tile)
-    const int vectors = sh.vectors;
-    if (vectors <= kList)
-        for (int i = tid; i < vectors; i += kThreads) {
-            const int first = c0 + sh.vector[i] * kVec;
-            const uint4 v = i < kNotes ? sh.note[i] : load_vector<T, ALIGNED>(row, first, end, a.vocab);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (noted > kNotesAll) sh.lost = true;
+    __syncwarp();
+    for (int i = lane; i < min(noted, kNotesAll) * kVectors; i += 32) {
+        const int note = i / kVectors, u = i % kVectors, of = sh.noted[warp][note];
+        const int first = c0 + ((of / kThreads * kVectors + u) * kThreads + of % kThreads) * kVec;
+        const uint4 v = note < kNotes ? sh.note[warp][note][u] : load_vector<T, ALIGNED>(row, first, end, a.vocab);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                const float2 f = pair_of<T>(w[e * 4 / kVec]);
-                const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
-                if (x >= bound && fabsf(x) < INFINITY) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(first + e));
-                }
+        for (int e = 0; e < kVec; ++e) {
+            const float2 f = pair_of<T>(w[e * 4 / kVec]);
+            const float x = sizeof(T) == 2 && (e & 1) ? f.y : f.x;
+            if (x >= bound && fabsf(x) < INFINITY) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kList) sh.list[at] = key_of(x, static_cast<uint32_t>(first + e));
             }
         }
+    }
 
     // ---- the chunk's sum, over the largest reference
     const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -488,8 +492,8 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) sh.warp_sum[warp] = total;
-    if (sh.count > 3 * kThreads || vectors > kList) {
-        const bool lost = sh.count > kList || vectors > kList;
+    if (sh.count > 3 * kThreads || sh.lost) {
+        const bool lost = sh.count > kList || sh.lost;
         __syncthreads();
         if (lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
         else trim_list(sh, k);      // more than ranking each takes
