@@ -16,8 +16,8 @@
 // logit, raised in front of the tiles 0, 3, 15, ..; what a thread has of a tile in which it sees a logit beyond the bound is noted (a
 // handful per tile) and looked at in the end, with the last bound.  No barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
-// The CTA that completes a group's counter merges its lists: the k-th largest of the lists' first candidates bounds what can be among
-// the k best, and the few that pass are ranked by counting.
+// The CTA that completes a group's counter merges its lists the same way: the k-th largest of the maxima over 128 shares of the entries
+// bounds what can be among the k best, and the few that pass are ranked by counting.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,8 +39,7 @@ constexpr int kEntries = 2048;              // candidates of all chunks of a gro
 constexpr int kMostChunks = 64;
 constexpr int kMostLists = 256;             // of a group
 constexpr int kFew = 256;                   // values that are ranked side by side
-constexpr int kCtas = 1036;                 // CTAs of 128 threads in a launch: seven per SM, all at the same time
-constexpr int kFewCtas = 148, kFewTiles = 4;
+constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
 
@@ -213,15 +212,15 @@ struct Shared {
             int noted[kWarps][kNotesAll];              // ... whose: tile * threads + thread
         };
         struct {                            // a group's lists
-            alignas(16) Key entry[kEntries];
-            alignas(16) Key value[kFew];
-            alignas(16) uint32_t front[128];           // largest values of shares of the lists' first candidates, as ordered words
+            Key entry[kEntries];
+            alignas(16) Key value[kFew];               // what may be among the k best
+            alignas(16) uint32_t front[128];           // largest values of shares of the entries, as ordered words
+            Key key[kFew];
             double sum[kMostLists], lse[kMostWidth], score[kMostWidth];
             float ref[kMostLists];
             int kind[kMostWidth];                      // 0 live, 1 finished, 2 dead
-            uint16_t passed[kEntries];
             uint8_t beam[kFew];
-            uint32_t least, top, low[kMostWidth];
+            uint32_t least, low[kMostWidth];
             int survivors, there;
         };
     };
@@ -516,9 +515,11 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     if (tid >= n && tid < k) out[tid] = 0;
 }
 
-// All lists of a group, by the CTA that finished its last chunk.
+// All lists of a group, by the CTA that finished its last chunk.  (It runs once: loops that are not unrolled come out ahead of the
+// instructions that an unrolled one would have to fetch.)
 static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     const wuda_beam_select_args& a = p.a;
+    constexpr int kParts = (kMostLists + kThreads - 1) / kThreads;
     const int tid = threadIdx.x, lane = tid & 31, k = a.k, chunks = p.chunks;
     const int per_beam = chunks * k, lists = a.width * chunks, entries = lists * k;
     const float by_beam = 1.f / per_beam;
@@ -526,14 +527,9 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     // ---- everything there is to read, then the beams' sums, eight lanes each
     const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
     const Partial* partials = p.partials + static_cast<int64_t>(g) * lists;
-    Key key[kEntries / kThreads];
-    constexpr int kParts = (kMostLists + kThreads - 1) / kThreads;
     float ref[kParts], score = 0.f;
     double sum[kParts];
     bool ended = false;
-#pragma unroll
-    for (int i = 0; i < kEntries / kThreads; ++i)
-        if (i * kThreads < entries) key[i] = i * kThreads + tid < entries ? __ldcg(keys + i * kThreads + tid) : 0;
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
         if (i * kThreads + tid < lists) ref[i] = __ldcg(&partials[i * kThreads + tid].ref), sum[i] = __ldcg(&partials[i * kThreads + tid].sum);
@@ -541,9 +537,15 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         score = a.scores[g * a.width + tid];
         ended = a.finished && a.finished[g * a.width + tid];
     }
+#pragma unroll 1
+    for (int e0 = tid; e0 < entries; e0 += 4 * kThreads) {
+        Key key[4];
 #pragma unroll
-    for (int i = 0; i < kEntries / kThreads; ++i)
-        if (i * kThreads + tid < entries) sh.entry[i * kThreads + tid] = key[i];
+        for (int u = 0; u < 4; ++u) key[u] = e0 + u * kThreads < entries ? __ldcg(keys + e0 + u * kThreads) : 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (e0 + u * kThreads < entries) sh.entry[e0 + u * kThreads] = key[u];
+    }
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
         if (i * kThreads + tid < lists) sh.ref[i * kThreads + tid] = ref[i], sh.sum[i * kThreads + tid] = sum[i];
@@ -552,7 +554,9 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         sh.score[tid] = score;
     }
     if (tid == 0) sh.survivors = sh.there = 0, sh.least = 0;
+    if (tid < 128) sh.front[tid] = 0;
     __syncthreads();
+#pragma unroll 1
     for (int w0 = 0; w0 < a.width; w0 += kThreads / 8) {
         const int w = w0 + tid / 8, at = min(w, a.width - 1) * chunks;
         float most = -FLT_MAX;
@@ -566,38 +570,38 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         if (w < a.width && (lane & 7) == 0) sh.lse[w] = most + log(total);      // (of a beam that was not read: not used)
     }
     __syncthreads();
+
     // ---- values as ordered words (0 none), in 64 bits where they are compared, in 32 where they are only bounded
     const auto value = [&](int e) -> Key {
         const Key key = sh.entry[e];
         const int w = beam_of(e);
-        if (sh.kind[w] == 1) return e == w * per_beam ? ordered(sh.score[w]) : 0;
+        if (sh.kind[w] == 1) return e == w * per_beam ? ordered(sh.score[w]) : 0;      // (its lists hold nothing)
         return sh.kind[w] == 0 && key ? ordered((sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w]) : 0;
     };
     const auto rounded = [](Key v) -> uint32_t { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
-    // the first `deep` of every list, at least k of them, better 4 k: the bound is then close to the k-th value
-    const int deep = min(k, (4 * k + lists - 1) / lists), pool = lists * deep;
-    uint32_t part = 0;      // the largest of a thread's share: 128 or more of them are at least 2 k
-    for (int i = tid; i < pool; i += kThreads) {
-        const int list = deep == 1 ? i : i / deep;
+    // the first of every list, 8 k or 256 together, in 128 shares (neighbours in a list in different ones): nothing below
+    // the k-th largest of the shares' largest is among the k best
+    const int deep = min(k, (max(8 * k, 256) + lists - 1) / lists);
+    const float by_deep = 1.f / deep;
+    uint32_t part = 0;
+#pragma unroll 1
+    for (int i = tid; i < lists * deep; i += kThreads) {
+        const int list = static_cast<int>((i + 0.5f) * by_deep);      // i / deep
         part = max(part, rounded(value(list * k + i - list * deep)));
     }
-    if constexpr (kThreads > 128) {
-#pragma unroll
-        for (int o = 1; o < kThreads / 128; o <<= 1) part = max(part, __shfl_xor_sync(0xffffffffu, part, o));
-    }
-    if (tid % (kThreads / 128) == 0) sh.front[tid / (kThreads / 128)] = part;
+    if (kThreads == 128) sh.front[tid] = part;
+    else if (part) atomicMax(&sh.front[tid % 128], part);
     __syncthreads();
-    // the k-th largest of them: nothing below it is among the k best
-    if (tid % (kThreads / 128) == 0) {
+    if (tid < 128) {
+        part = sh.front[tid];
         int larger = 0, not_smaller = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (int i = 0; i < 128; i += 4) {
             const uint4 other = *reinterpret_cast<const uint4*>(&sh.front[i]);
             larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
             not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
         }
         if (larger < k && k <= not_smaller) sh.least = part;
-        if (larger == 0) sh.top = part;
     }
     __syncthreads();
     const uint32_t least = max(sh.least, 1u);
@@ -608,82 +612,55 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         sh.low[tid] = sh.kind[tid] == 0 ? (least > 1u && low == low ? ordered(low) : 1u) : sh.kind[tid] == 1 ? 0u : 0xffffffffu;
     }
     __syncthreads();
+    const auto pass = [&](int e, Key v) {
+        const int at = atomicAdd(&sh.survivors, 1);
+        if (at < kFew) sh.value[at] = v, sh.key[at] = sh.entry[e], sh.beam[at] = static_cast<uint8_t>(beam_of(e));
+    };
 #pragma unroll 4
     for (int e = tid; e < entries; e += kThreads) {
-        const int w = beam_of(e);
-        if (static_cast<uint32_t>(sh.entry[e] >> 32) < sh.low[w]) continue;
+        if (static_cast<uint32_t>(sh.entry[e] >> 32) < sh.low[beam_of(e)]) continue;
         const Key v = value(e);
-        if (rounded(v) < least) continue;
-        const int at = atomicAdd(&sh.survivors, 1);
-        sh.passed[at] = static_cast<uint16_t>(e);
-        if (at < kFew) sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(w);
+        if (rounded(v) >= least) pass(e, v);
     }
     __syncthreads();
     int n = sh.survivors;
-    if (n > 2 * k + 32) {
-        // a few beams have most of the best: the k-th largest value of what passed, exactly but for its rounding
-        uint32_t mine[kEntries / kThreads];
-#pragma unroll
-        for (int i = 0; i < kEntries / kThreads; ++i)
-            if (i * kThreads < n) mine[i] = i * kThreads + tid < n ? rounded(value(sh.passed[i * kThreads + tid])) : 0;
-        const uint32_t bound = static_cast<uint32_t>(kth_largest(k, least, sh.top, sh.hits, [&](const auto& f) {
-#pragma unroll
-            for (int i = 0; i < kEntries / kThreads; ++i)
-                if (i * kThreads < n) f(static_cast<Key>(mine[i]));
-        }));
-        uint16_t entry[kEntries / kThreads];
-#pragma unroll
-        for (int i = 0; i < kEntries / kThreads; ++i)
-            if (i * kThreads + tid < n) entry[i] = sh.passed[i * kThreads + tid];
-        if (tid == 0) sh.survivors = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kEntries / kThreads; ++i) {
-            if (i * kThreads + tid >= n || mine[i] < bound) continue;
-            const int at = atomicAdd(&sh.survivors, 1);
-            sh.passed[at] = entry[i];
-            if (at < kFew) sh.value[at] = value(entry[i]), sh.beam[at] = static_cast<uint8_t>(beam_of(entry[i]));
-        }
-        __syncthreads();
-        n = sh.survivors;
-    }
     if (n > kFew) {
         // many equal values: the k best by value, then by beam, then by logit and token
-        const auto mine = [&](const auto& f) {
-            for (int i = tid; i < n; i += kThreads) f(static_cast<int>(sh.passed[i]));
+        const auto all = [&](const auto& f) {      // f(entry, value, beam)
+#pragma unroll 1
+            for (int e = tid; e < entries; e += kThreads)
+                if (const Key v = value(e)) f(e, v, beam_of(e));
         };
-        const Key worst = kth_largest(k, 0, ~0ull, sh.hits, [&](const auto& f) { mine([&](int e) { f(value(e)); }); });
         const auto count = [&](const auto& test) {
             int c = 0;
-            mine([&](int e) { c += test(e); });
+            all([&](int e, Key v, int w) { c += test(e, v, w); });
             start_totals(sh.hits);
             return block_total(c, sh.hits, 0);
         };
-        int wanted = k - count([&](int e) { return value(e) > worst; });
+        const Key worst = kth_largest(k, 0, ~0ull, sh.hits, [&](const auto& f) { all([&](int, Key v, int) { f(v); }); });
+        int wanted = k - count([&](int, Key v, int) { return v > worst; });
         const int beam = 31 - static_cast<int>(kth_largest(wanted, 0, 31, sh.hits, [&](const auto& f) {
-            mine([&](int e) { if (value(e) == worst) f(static_cast<Key>(31 - beam_of(e))); });
+            all([&](int, Key v, int w) { if (v == worst) f(static_cast<Key>(31 - w)); });
         }));
-        wanted -= count([&](int e) { return value(e) == worst && beam_of(e) < beam; });
+        wanted -= count([&](int, Key v, int w) { return v == worst && w < beam; });
         const Key last = kth_largest(wanted, 0, ~0ull, sh.hits, [&](const auto& f) {
-            mine([&](int e) { if (value(e) == worst && beam_of(e) == beam) f(sh.entry[e]); });
+            all([&](int e, Key v, int w) { if (v == worst && w == beam) f(sh.entry[e]); });
         });
+        __syncthreads();
         if (tid == 0) sh.survivors = 0;
         __syncthreads();
-        for (int e = tid; e < entries; e += kThreads) {
-            const Key v = value(e);
-            const int w = beam_of(e);
-            if (v == 0 || v < worst || (v == worst && (w > beam || (w == beam && sh.entry[e] < last)))) continue;
-            const int at = atomicAdd(&sh.survivors, 1);
-            if (at < kFew) sh.passed[at] = static_cast<uint16_t>(e), sh.value[at] = v, sh.beam[at] = static_cast<uint8_t>(w);
-        }
+        all([&](int e, Key v, int w) {
+            if (v > worst || (v == worst && (w < beam || (w == beam && sh.entry[e] >= last)))) pass(e, v);
+        });
         __syncthreads();
-        n = min(sh.survivors, kFew);
+        n = min(sh.survivors, kFew);      // (k of them)
     }
-    // their order: larger value, lower beam; within a beam larger logit, lower token
+
+    // ---- their order: larger value, lower beam; within a beam larger logit, lower token
     for (int i = tid; i < n; i += kThreads) {
-        const Key v = sh.value[i], key = sh.entry[sh.passed[i]];
+        const Key v = sh.value[i], mine = sh.key[i];
         const int w = sh.beam[i];
-        const auto before = [&](int j) { return sh.beam[j] != w ? sh.beam[j] < w : sh.entry[sh.passed[j]] > key; };
+        const auto before = [&](int j) { return sh.beam[j] != w ? sh.beam[j] < w : sh.key[j] > mine; };
         int rank = 0, equal = 0, j = 0;
         uint32_t ties[2] = {0, 0};      // among the first 64
 #pragma unroll 4
@@ -709,7 +686,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         atomicAdd(&sh.there, 1);
         const int64_t at = static_cast<int64_t>(g) * k + rank;
         const bool done = sh.kind[w] == 1;
-        const int token = done ? a.eos_token : static_cast<int>(token_of(key));
+        const int token = done ? a.eos_token : static_cast<int>(token_of(mine));
         a.scores_out[at] = static_cast<float>(unordered(v));
         a.parents_out[at] = w;
         a.tokens_out[at] = token;
@@ -748,23 +725,26 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
     B::merge(sh, p, g);
 }
 
-// How the rows are cut: chunks of whole tiles, as many as CTAs of 128 threads are resident on the device together, and lists that the
-// merge can hold.  Where that leaves less than a warp per scheduler and several tiles per CTA, CTAs of 512 threads.
+// How the rows are cut, into chunks of whole tiles and lists that the merge can hold.
+//   Up to 148 rows of more work than a tile of 128 threads per SM: CTAs of 512 threads, one per SM at most.  Fewer and longer lists make
+//   the merge shorter, and a CTA alone on its SM needs the threads.  8 rows x 131072 bf16, k = 16: 10.3 us (12.9 in CTAs of 128), 128
+//   rows x 65536 fp32, k = 32: 18.7 (22.2); 64 rows x 131072 fp32, k = 4: 15.5 (15.3).
+//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 37.4 us in two chunks a row,
+//   40.2 in three, 50.1 with 512 threads; 4 rows x 32000 bf16: 9.0 us in eight chunks of a tile (9.6 with 512 threads).
 struct Cut {
     int threads, chunks, chunk_vectors;
 };
 Cut cut(int groups, int width, int vocab, int k, int type) {
-    const int rows = groups * width;
+    const int rows = groups * width, of_128 = (type == 2 ? 4 : 8) * kVectors * 128;
     Cut c = {};
-    for (c.threads = 128;; c.threads = 512) {
-        const int tile = (type == 2 ? 4 : 8) * c.threads * kVectors, tiles = (vocab + tile - 1) / tile;
-        int n = std::max(kCtas / (c.threads / 128) / rows, 1);
-        n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
-        const int per = (tiles + n - 1) / n;
-        c.chunks = (tiles + per - 1) / per;
-        c.chunk_vectors = per * c.threads * kVectors;
-        if (c.threads == 512 || per < kFewTiles || rows * c.chunks >= kFewCtas) return c;
-    }
+    c.threads = rows <= kSms && static_cast<int64_t>(rows) * ((vocab + of_128 - 1) / of_128) > kSms ? 512 : 128;
+    const int tile = of_128 * (c.threads / 128), tiles = (vocab + tile - 1) / tile;
+    int n = std::max((c.threads == 512 ? 1 : 7) * kSms / rows, 1);
+    n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
+    const int per = (tiles + n - 1) / n;
+    c.chunks = (tiles + per - 1) / per;
+    c.chunk_vectors = per * c.threads * kVectors;
+    return c;
 }
 
 bool sizes_fit(int groups, int width, int vocab, int k, int type) {
