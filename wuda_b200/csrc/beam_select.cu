@@ -38,7 +38,7 @@ constexpr int kNotesOfBlock = 160, kNotesAllOfBlock = 1024; // notes of a CTA's 
 constexpr int kEntries = 2048;              // candidates of all chunks of a group
 constexpr int kMostChunks = 64;
 constexpr int kMostLists = 256;             // of a group
-constexpr int kFew = 256;                   // values that are ranked side by side
+constexpr int kFew = 512;                   // values that are ranked side by side
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 40.f;               // e^40 * 2^24 elements are far from the largest fp32
@@ -112,48 +112,43 @@ __device__ __forceinline__ uint4 load16(const void* p) {
     return v;
 }
 
-// Elements [at, at + kVec) of a row; masked from `end` on.  ALIGNED: the row lies on 16 bytes.  Otherwise two aligned loads, both within
-// the row [0, vocab), are shifted together.
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ uint4 load_vector(const T* __restrict__ row, int at, int end, int vocab) {
-    constexpr int kVec = Type<T>::kVec;
-    const T* p = row + at;
-    if (at + kVec <= end) {
-        if (ALIGNED) return load16(p);
-        const uintptr_t address = reinterpret_cast<uintptr_t>(p);
-        const int off = static_cast<int>(address & 15);
-        const T* low = reinterpret_cast<const T*>(address - off);
-        if (off == 0) return load16(p);
-        if (low >= row && low + 2 * kVec <= row + vocab) {
-            const uint4 a = load16(low), b = load16(low + kVec);
-            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (off & 8) {
+// Elements [at, at + kVec) of a row one by one, masked where they are not in [0, vocab).
+template <typename T>
+__device__ __noinline__ uint4 load_elements(const T* row, int at, int vocab) {
+    uint32_t w[4] = {Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked};
 #pragma unroll
-                for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-            }
-            if (off & 4) {
-#pragma unroll
-                for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-            }
-            const int bits = (off & 3) * 8;
-            return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
-                              __funnelshift_r(w[3], w[4], bits));
+    for (int i = 0; i < Type<T>::kVec; ++i) {
+        if (at + i < 0 || at + i >= vocab) continue;
+        if constexpr (sizeof(T) == 4) {
+            w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
+        } else {
+            const uint32_t x = reinterpret_cast<const uint16_t*>(row)[at + i];
+            w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (x << 16) : (w[i / 2] & 0xffff0000u) | x;
         }
     }
-    uint32_t w[4] = {Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked};
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at + i < end) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (at + i < end) {
-                const uint32_t x = reinterpret_cast<const uint16_t*>(p)[i];
-                w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (x << 16) : (w[i / 2] & 0xffff0000u) | x;
-            }
-    }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The same sixteen bytes at a time, where row + at lies on 16 bytes (ALIGNED) or from the two such pieces that it lies in.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_vector(const T* row, int at, int vocab) {
+    constexpr int kVec = Type<T>::kVec;
+    if (at >= vocab) return make_uint4(Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked, Type<T>::kMasked);
+    const int off = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row + at) & 15), low = at - off / static_cast<int>(sizeof(T));
+    if (off == 0 && at >= 0 && at + kVec <= vocab) return load16(row + at);
+    if (off == 0 || low < 0 || low + 2 * kVec > vocab) return load_elements(row, at, vocab);
+    const uint4 a = load16(row + low), b = load16(row + low + kVec);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (off & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int bits = (off & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                      __funnelshift_r(w[3], w[4], bits));
 }
 
 // NaN -> -inf in all elements of a word, and a word's elements as fp32
@@ -208,19 +203,19 @@ struct Shared {
         struct {                            // a chunk
             alignas(16) Key list[kList];
             alignas(16) uint4 note[kWarps][kNotes][kVectors];      // what a thread had of a tile in which a logit passed the bound
-            alignas(16) float part_max[128];           // maxima of parts of the tiles
-            int noted[kWarps][kNotesAll];              // ... whose: tile * threads + thread
+            alignas(16) uint32_t part_max[128];        // maxima of parts of the tiles, as ordered words
+            int noted[kWarps][kNotesAll];              // ... whose: tile * 32 + lane
+            float noted_top[kWarps][kNotesAll];        // ... and the largest logit of it
         };
         struct {                            // a group's lists
             Key entry[kEntries];
             alignas(16) Key value[kFew];               // what may be among the k best
             alignas(16) uint32_t front[128];           // largest values of shares of the entries, as ordered words
-            Key key[kFew];
+            alignas(16) Key tie[kFew];                 // ... and what decides between equal ones
             double sum[kMostLists], lse[kMostWidth], score[kMostWidth];
             float ref[kMostLists];
             int kind[kMostWidth];                      // 0 live, 1 finished, 2 dead
-            uint8_t beam[kFew];
-            uint32_t least, low[kMostWidth];
+            uint32_t least, top, low[kMostWidth];
             int survivors, there;
         };
     };
@@ -309,7 +304,7 @@ static __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row,
     Key least = 0;
     for (int at = c0; at < end; at += kThreads * kVec) {
         const int first = at + threadIdx.x * kVec;
-        const uint4 v = load_vector<T, false>(row, first, end, vocab);
+        const uint4 v = load_elements(row, first, vocab);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         Key keys[kVec];
         bool above = false;
@@ -328,22 +323,18 @@ static __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row,
     }
 }
 
-// The k-th largest of 64 (k <= 32) or 128 maxima, of as many groups of neighbouring threads over all that they have seen: k logits so
-// far are at or above it.
+// The k-th largest of 64 (k <= 32) or 128 maxima, each over all that some threads have seen: k logits so far are at or above it.
 static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
     const int tid = threadIdx.x, parts = k <= 32 ? 64 : 128, by = kThreads / parts;
-    float part = so_far;
-#pragma unroll
-    for (int o = 1; o < kThreads / 64; o <<= 1)
-        if (o < by) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, o));
-    if (tid % by == 0) sh.part_max[tid / by] = part;
+    atomicMax(&sh.part_max[tid % parts], ordered(so_far));      // (what was there is of earlier tiles)
     __syncthreads();
-    int larger = 0, not_smaller = 0;      // than the group's maximum; each of its threads counts a share of them
+    const uint32_t part = sh.part_max[tid / by];
+    int larger = 0, not_smaller = 0;      // than this part; each of `by` threads counts a share of them
     const int n = parts / 4 / by;
-    const float4* share = reinterpret_cast<const float4*>(sh.part_max) + tid % by * n;
+    const uint4* share = reinterpret_cast<const uint4*>(sh.part_max) + tid % by * n;
 #pragma unroll 8
     for (int i = 0; i < n; ++i) {
-        const float4 other = share[i];
+        const uint4 other = share[i];
         larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
         not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
     }
@@ -351,7 +342,7 @@ static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, in
 #pragma unroll
     for (int o = 1; o < kThreads / 64; o <<= 1)
         if (o < by) both += __shfl_xor_sync(0xffffffffu, both, o);
-    if ((both & 0xffff) < k && k <= both >> 16) sh.bound = part;      // (equal ones write the same)
+    if ((both & 0xffff) < k && k <= both >> 16) sh.bound = unordered(part);      // (equal ones write the same)
     __syncthreads();
     *raised = sh.bound > bound;
     return sh.bound;
@@ -369,17 +360,51 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
         sh.lost = false;
         sh.bound = -INFINITY;
     }
+    if (tid < 128) sh.part_max[tid] = ordered(-INFINITY);
+    __syncthreads();
     constexpr int kTile = kThreads * kVectors * kVec;
-    const int tiles = (end - c0 + kTile - 1) / kTile;
-    uint4 next[kVectors];
+    const int tiles = (end - c0 + kTile - 1) / kTile, whole = (end - c0) / kTile;
+    // A row's last, partial tile is spread over the threads, a vector each first, so that there are maxima of many parts of it.  In a
+    // whole tile a warp's part is contiguous, vector after vector.  Where the row does not lie on 16 bytes, what is loaded are the aligned
+    // 16 bytes in which a vector begins; its end is in the next lane's (for the last lane: in lane 0's next, and one more load of lane 0's).
+    const int off = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15), back = off / static_cast<int>(sizeof(T));
+    const auto element_of = [&](int tile, int u, int of_lane) {
+        const int at = tile < whole ? (warp * kVectors + u) * 32 : u * kThreads + warp * 32;
+        return c0 + (tile * kThreads * kVectors + at + of_lane) * kVec;
+    };
+    uint4 next[kVectors + !ALIGNED];
     const auto fetch = [&](int tile) {
-        const int at = c0 + tile * kTile + tid * kVec;
-        if (ALIGNED && c0 + (tile + 1) * kTile <= end) {
+        if (tile >= whole) {
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u) next[u] = load16(row + at + u * kThreads * kVec);
-        } else {
+            for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, element_of(tile, u, lane), a.vocab);
+            return;
+        }
+        const int at = element_of(tile, 0, lane) - back;
+        if (at - lane * kVec >= 0 && at + (kVectors * 32 + !ALIGNED - lane) * kVec <= a.vocab) {      // (of the whole warp)
 #pragma unroll
-            for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, ALIGNED>(row, at + u * kThreads * kVec, end, a.vocab);
+            for (int u = 0; u < kVectors; ++u) next[u] = load16(row + at + u * 32 * kVec);
+            if constexpr (!ALIGNED) {
+                if (lane == 0) next[kVectors] = load16(row + at + kVectors * 32 * kVec);
+            }
+        } else if constexpr (!ALIGNED) {      // the row's first bytes or last ones
+#pragma unroll
+            for (int u = 0; u < kVectors; ++u) next[u] = load_vector<T, true>(row, at + u * 32 * kVec, a.vocab);
+            if (lane == 0) next[kVectors] = load_vector<T, true>(row, at + kVectors * 32 * kVec, a.vocab);
+        }
+    };
+    // the words of a thread's vectors from what was loaded: SKIP whole words and off % 4 bytes of each are left out
+    const auto shifted = [&](uint32_t (&w)[4 * kVectors], auto skip) {
+        constexpr int SKIP = decltype(skip)::value;
+        const int bits = (off & 3) * 8;
+#pragma unroll
+        for (int u = 0; u < kVectors; ++u) {
+            const uint4 now = next[u], then = next[kVectors + !ALIGNED - 1 < u + 1 ? u : u + 1];
+            uint32_t x[8] = {now.x, now.y, now.z, now.w};
+            const uint32_t give[4] = {lane ? now.x : then.x, lane ? now.y : then.y, lane ? now.z : then.z, lane ? now.w : then.w};
+#pragma unroll
+            for (int i = 0; i <= SKIP; ++i) x[4 + i] = __shfl_sync(0xffffffffu, give[i], lane + 1);      // (of lane 0 for lane 31)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[4 * u + i] = __funnelshift_r(x[SKIP + i], x[SKIP + i + 1], bits);
         }
     };
     if (a.finished && a.finished[row_number]) return;
@@ -388,14 +413,22 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
     int noted = 0;        // of the warp's vectors
-    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, ..
+    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, .. or 0, 1, 3, 7, ..
     for (int tile = 0; tile < tiles; ++tile) {
         uint32_t w[4 * kVectors];
+        if (ALIGNED || off == 0 || tile >= whole) {
 #pragma unroll
-        for (int u = 0; u < kVectors; ++u) {      // masked tokens are -inf from here on
-            w[4 * u] = without_nan<T>(next[u].x), w[4 * u + 1] = without_nan<T>(next[u].y);
-            w[4 * u + 2] = without_nan<T>(next[u].z), w[4 * u + 3] = without_nan<T>(next[u].w);
+            for (int u = 0; u < kVectors; ++u) w[4 * u] = next[u].x, w[4 * u + 1] = next[u].y, w[4 * u + 2] = next[u].z, w[4 * u + 3] = next[u].w;
+        } else if constexpr (!ALIGNED) {
+            switch (off >> 2) {      // (the same for the whole row)
+                case 0: shifted(w, std::integral_constant<int, 0>()); break;
+                case 1: shifted(w, std::integral_constant<int, 1>()); break;
+                case 2: shifted(w, std::integral_constant<int, 2>()); break;
+                default: shifted(w, std::integral_constant<int, 3>());
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4 * kVectors; ++i) w[i] = without_nan<T>(w[i]);      // masked tokens are -inf from here on
         if (tile + 1 < tiles) fetch(tile + 1);
         // ---- the maximum
         const auto maximum = [&] {
@@ -440,14 +473,14 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
         so_far = fmaxf(so_far, top);
         bool with_equal = false;      // a logit equal to the bound is a candidate where the bound is this tile's
         if (tile == refresh) {
-            refresh = 4 * refresh + 3;
+            refresh = k <= 32 ? 4 * refresh + 3 : 2 * refresh + 1;
             bound = raise_bound(sh, so_far, k, bound, &with_equal);
         }
         const bool hit = with_equal ? top >= bound : top > bound;
         const uint32_t hits = __ballot_sync(0xffffffffu, hit);
         if (hits) {      // places without atomics: each warp has a list of its own
             const int at = noted + __popc(hits & ((1u << lane) - 1));
-            if (hit && at < kNotesAll) sh.noted[warp][at] = tile * kThreads + tid;
+            if (hit && at < kNotesAll) sh.noted[warp][at] = tile * 32 + lane, sh.noted_top[warp][at] = top;
             if (hit && at < kNotes) {
 #pragma unroll
                 for (int u = 0; u < kVectors; ++u) sh.note[warp][at][u] = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
@@ -458,14 +491,23 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
 
     // ---- candidates: the noted elements that pass the last bound
     bool raised;
-    if (4 * (tiles - 1) + 3 != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
+    if ((k <= 32 ? 4 * (tiles - 1) + 3 : 2 * (tiles - 1) + 1) != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
     else __syncthreads();      // (it was raised with the last tile)
     if (noted > kNotesAll) sh.lost = true;
     __syncwarp();
-    for (int i = lane; i < min(noted, kNotesAll) * kVectors; i += 32) {
-        const int note = i / kVectors, u = i % kVectors, of = sh.noted[warp][note];
-        const int first = c0 + ((of / kThreads * kVectors + u) * kThreads + of % kThreads) * kVec;
-        const uint4 v = note < kNotes ? sh.note[warp][note][u] : load_vector<T, ALIGNED>(row, first, end, a.vocab);
+    int kept = 0;         // the notes that do, to the front of the list
+    for (int i = 0; i < min(noted, kNotesAll); i += 32) {
+        const bool keep = i + lane < min(noted, kNotesAll) && sh.noted_top[warp][i + lane] >= bound;
+        const int of = keep ? sh.noted[warp][i + lane] : 0;
+        const uint32_t keeps = __ballot_sync(0xffffffffu, keep);
+        if (keep) sh.noted[warp][kept + __popc(keeps & ((1u << lane) - 1))] = of | (i + lane < kNotes ? (i + lane + 1) << 24 : 0);
+        kept += __popc(keeps);
+    }
+    __syncwarp();
+    for (int i = lane; i < kept * kVectors; i += 32) {
+        const int u = i % kVectors, of = sh.noted[warp][i / kVectors], note = (of >> 24) - 1, from = of & 0xffffff;
+        const int first = element_of(from / 32, u, from % 32);
+        const uint4 v = note >= 0 ? sh.note[warp][note][u] : load_vector<T, ALIGNED>(row, first, a.vocab);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < kVec; ++e) {
@@ -579,9 +621,9 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         return sh.kind[w] == 0 && key ? ordered((sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w]) : 0;
     };
     const auto rounded = [](Key v) -> uint32_t { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
-    // the first of every list, 8 k or 256 together, in 128 shares (neighbours in a list in different ones): nothing below
+    // the first of every list, 16 k or 256 together, in 128 shares (neighbours in a list in different ones): nothing below
     // the k-th largest of the shares' largest is among the k best
-    const int deep = min(k, (max(8 * k, 256) + lists - 1) / lists);
+    const int deep = min(k, (max(16 * k, 256) + lists - 1) / lists);
     const float by_deep = 1.f / deep;
     uint32_t part = 0;
 #pragma unroll 1
@@ -602,6 +644,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
             not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
         }
         if (larger < k && k <= not_smaller) sh.least = part;
+        if (larger == 0) sh.top = part;
     }
     __syncthreads();
     const uint32_t least = max(sh.least, 1u);
@@ -614,7 +657,8 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     __syncthreads();
     const auto pass = [&](int e, Key v) {
         const int at = atomicAdd(&sh.survivors, 1);
-        if (at < kFew) sh.value[at] = v, sh.key[at] = sh.entry[e], sh.beam[at] = static_cast<uint8_t>(beam_of(e));
+        // lower beam; within a beam larger logit, lower token (tokens have 24 bits)
+        if (at < kFew) sh.value[at] = v, sh.tie[at] = static_cast<Key>(31 - beam_of(e)) << 56 | sh.entry[e] >> 32 << 24 | (sh.entry[e] & 0xffffff);
     };
 #pragma unroll 4
     for (int e = tid; e < entries; e += kThreads) {
@@ -624,6 +668,25 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     }
     __syncthreads();
     int n = sh.survivors;
+    if (n > kFew) {
+        // a few beams have most of the best: the k-th largest value, exactly but for its rounding
+        uint32_t mine[kEntries / kThreads];
+#pragma unroll
+        for (int i = 0; i < kEntries / kThreads; ++i) mine[i] = i * kThreads + tid < entries ? rounded(value(i * kThreads + tid)) : 0;
+        const uint32_t bound = static_cast<uint32_t>(kth_largest(k, least, sh.top, sh.hits, [&](const auto& f) {
+#pragma unroll
+            for (int i = 0; i < kEntries / kThreads; ++i)
+                if (i * kThreads < entries) f(static_cast<Key>(mine[i]));
+        }));
+        __syncthreads();
+        if (tid == 0) sh.survivors = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEntries / kThreads; ++i)
+            if (mine[i] && mine[i] >= bound) pass(i * kThreads + tid, value(i * kThreads + tid));
+        __syncthreads();
+        n = sh.survivors;
+    }
     if (n > kFew) {
         // many equal values: the k best by value, then by beam, then by logit and token
         const auto all = [&](const auto& f) {      // f(entry, value, beam)
@@ -656,37 +719,22 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         n = min(sh.survivors, kFew);      // (k of them)
     }
 
-    // ---- their order: larger value, lower beam; within a beam larger logit, lower token
+    // ---- their order
     for (int i = tid; i < n; i += kThreads) {
-        const Key v = sh.value[i], mine = sh.key[i];
-        const int w = sh.beam[i];
-        const auto before = [&](int j) { return sh.beam[j] != w ? sh.beam[j] < w : sh.key[j] > mine; };
-        int rank = 0, equal = 0, j = 0;
-        uint32_t ties[2] = {0, 0};      // among the first 64
+        const Key v = sh.value[i], tie = sh.tie[i];
+        int rank = 0, j = 0;
 #pragma unroll 4
         for (; j + 1 < n; j += 2) {
-            const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.value[j]);
-            rank += (other.x > v) + (other.y > v);
-            const uint32_t same = (other.x == v) | (other.y == v) << 1;
-            equal += __popc(same);
-            if (j < 64) ties[0] |= j < 32 ? same << j : 0, ties[1] |= j < 32 ? 0 : same << (j - 32);
+            const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(&sh.value[j]), ties = *reinterpret_cast<const ulonglong2*>(&sh.tie[j]);
+            rank += (other.x > v || (other.x == v && ties.x > tie)) + (other.y > v || (other.y == v && ties.y > tie));
         }
-        if (j < n) {
-            const uint32_t same = sh.value[j] == v;
-            rank += sh.value[j] > v, equal += same;
-            if (j < 64) ties[0] |= j < 32 ? same << j : 0, ties[1] |= j < 32 ? 0 : same << (j - 32);
-        }
-        if (equal > 1) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                for (uint32_t m = ties[t]; m; m &= m - 1) rank += before(t * 32 + __ffs(m) - 1);
-            for (j = 64; j < n; ++j) rank += sh.value[j] == v && before(j);
-        }
+        if (j < n) rank += sh.value[j] > v || (sh.value[j] == v && sh.tie[j] > tie);
         if (rank >= k) continue;
         atomicAdd(&sh.there, 1);
         const int64_t at = static_cast<int64_t>(g) * k + rank;
+        const int w = 31 - static_cast<int>(tie >> 56);
         const bool done = sh.kind[w] == 1;
-        const int token = done ? a.eos_token : static_cast<int>(token_of(mine));
+        const int token = done ? a.eos_token : static_cast<int>(~tie & 0xffffff);
         a.scores_out[at] = static_cast<float>(unordered(v));
         a.parents_out[at] = w;
         a.tokens_out[at] = token;
@@ -702,7 +750,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
 }
 };
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool ALIGNED>
 __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(const __grid_constant__ Params p) {
     using B = Block<kThreads>;
     __shared__ typename B::Shared sh;
@@ -711,8 +759,7 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int number = blockIdx.x % p.chunks, row = blockIdx.x / p.chunks, g = row / a.width;
     const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
-    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) B::template chunk<T, true>(sh, p, x, row, number);
-    else B::template chunk<T, false>(sh, p, x, row, number);
+    B::template chunk<T, ALIGNED>(sh, p, x, row, number);
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -793,10 +840,16 @@ extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream)
     const int64_t parts = static_cast<int64_t>(a.groups) * a.width * p.chunks;
     p.partials = static_cast<Partial*>(a.workspace);
     p.lists = reinterpret_cast<Key*>(p.partials + parts);
-    static void (*const kernels[2][3])(Params) = {
-        {beam_select_kernel<__nv_bfloat16, 128>, beam_select_kernel<__half, 128>, beam_select_kernel<float, 128>},
-        {beam_select_kernel<__nv_bfloat16, 512>, beam_select_kernel<__half, 512>, beam_select_kernel<float, 512>}};
-    WUDA_CUDA(launch_pdl(kernels[c.threads == 512][a.logits_type], dim3(static_cast<unsigned>(parts)), dim3(c.threads), 0,
+    // whether all rows lie on 16 bytes
+    const int64_t in_16 = a.logits_type == 2 ? 4 : 8;
+    const bool aligned = aligned16(a.logits) && (a.width == 1 || a.beam_stride % in_16 == 0) && (a.groups == 1 || a.group_stride % in_16 == 0);
+    using Kernel = void (*)(Params);
+    static const Kernel kernels[2][2][3] = {
+        {{beam_select_kernel<__nv_bfloat16, 128, false>, beam_select_kernel<__half, 128, false>, beam_select_kernel<float, 128, false>},
+         {beam_select_kernel<__nv_bfloat16, 512, false>, beam_select_kernel<__half, 512, false>, beam_select_kernel<float, 512, false>}},
+        {{beam_select_kernel<__nv_bfloat16, 128, true>, beam_select_kernel<__half, 128, true>, beam_select_kernel<float, 128, true>},
+         {beam_select_kernel<__nv_bfloat16, 512, true>, beam_select_kernel<__half, 512, true>, beam_select_kernel<float, 512, true>}}};
+    WUDA_CUDA(launch_pdl(kernels[aligned][c.threads == 512][a.logits_type], dim3(static_cast<unsigned>(parts)), dim3(c.threads), 0,
                          static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }
