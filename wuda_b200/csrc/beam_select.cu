@@ -774,10 +774,11 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
 
 // How the rows are cut, into chunks of whole tiles and lists that the merge can hold.
 //   Up to 148 rows of more work than a tile of 128 threads per SM: CTAs of 512 threads, one per SM at most.  Fewer and longer lists make
-//   the merge shorter, and a CTA alone on its SM needs the threads.  8 rows x 131072 bf16, k = 16: 10.3 us (12.9 in CTAs of 128), 128
-//   rows x 65536 fp32, k = 32: 18.7 (22.2); 64 rows x 131072 fp32, k = 4: 15.5 (15.3).
-//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 37.4 us in two chunks a row,
-//   40.2 in three, 50.1 with 512 threads; 4 rows x 32000 bf16: 9.0 us in eight chunks of a tile (9.6 with 512 threads).
+//   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 12.3 us (14.2 in CTAs of 128), 128 rows x
+//   131072 bf16, k = 16: 17.6 (19.8); 64 rows x 131072 fp32, k = 4: 15.8 (16.0).
+//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 36.7 us in two chunks a row,
+//   39.0 in three, 49.3 with 512 threads; 4 rows x 32000 bf16: 8.7 us in eight chunks of a tile (9.6 with 512 threads).  Rows that
+//   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 55.3 -> 44.0 us.
 struct Cut {
     int threads, chunks, chunk_vectors;
 };
@@ -786,7 +787,9 @@ Cut cut(int groups, int width, int vocab, int k, int type) {
     Cut c = {};
     c.threads = rows <= kSms && static_cast<int64_t>(rows) * ((vocab + of_128 - 1) / of_128) > kSms ? 512 : 128;
     const int tile = of_128 * (c.threads / 128), tiles = (vocab + tile - 1) / tile;
-    int n = std::max((c.threads == 512 ? 1 : 7) * kSms / rows, 1);
+    const int resident = (c.threads == 512 ? 1 : 7) * kSms;
+    int n = std::max(resident / rows, 1);
+    if (n == 1 && rows * 5 < resident * 4 && tiles >= 6) n = 3;
     n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
     const int per = (tiles + n - 1) / n;
     c.chunks = (tiles + per - 1) / per;
