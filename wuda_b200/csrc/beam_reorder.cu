@@ -34,9 +34,16 @@ struct Params {
 
 inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (8ull * rows + capacity); }
 
-__device__ __forceinline__ int lowest_but(uint32_t set, int n) {      // the n-th lowest member, -1 where there are fewer
-    for (; n > 0 && set; --n) set &= set - 1;
-    return set ? __ffs(set) - 1 : -1;
+// The n-th lowest member of a set, -1 where there are fewer: halves, by their members.
+__device__ __forceinline__ int lowest_but(uint32_t set, int n) {
+    if (n >= __popc(set)) return -1;
+    int at = 0;
+#pragma unroll
+    for (int half = 16; half; half >>= 1) {
+        const int below = __popc(set & ((1u << half) - 1));
+        if (n >= below) n -= below, set >>= half, at += half;
+    }
+    return at;
 }
 
 struct Span {
