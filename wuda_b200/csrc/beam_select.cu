@@ -194,7 +194,7 @@ static constexpr int kWarps = kThreads / 32, kNotes = kNotesOfBlock / kWarps, kN
 struct Shared {
     int count;                              // candidates (those beyond kList are lost)
     bool lost;                              // more was to be noted than there are places for
-    float bound;                            // the k-th largest logit so far, or less
+    uint32_t bound, highest;                // the k-th largest logit so far, or less, and the largest, as ordered words
     int hits[3];
     float warp_ref[kWarps];
     double warp_sum[kWarps];
@@ -215,7 +215,7 @@ struct Shared {
             double sum[kMostLists], lse[kMostWidth], score[kMostWidth];
             float ref[kMostLists];
             int kind[kMostWidth];                      // 0 live, 1 finished, 2 dead
-            uint32_t least, top, low[kMostWidth];
+            uint32_t low[kMostWidth];
             int survivors, there;
         };
     };
@@ -323,16 +323,14 @@ static __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row,
     }
 }
 
-// The k-th largest of 64 (k <= 32) or 128 maxima, each over all that some threads have seen: k logits so far are at or above it.
-static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
-    const int tid = threadIdx.x, parts = k <= 32 ? 64 : 128, by = kThreads / parts;
-    atomicMax(&sh.part_max[tid % parts], ordered(so_far));      // (what was there is of earlier tiles)
-    __syncthreads();
-    const uint32_t part = sh.part_max[tid / by];
-    int larger = 0, not_smaller = 0;      // than this part; each of `by` threads counts a share of them
-    const int n = parts / 4 / by;
-    const uint4* share = reinterpret_cast<const uint4*>(sh.part_max) + tid % by * n;
-#pragma unroll 8
+// The k-th largest of 64 (k <= 32) or 128 words goes to *kth, the largest to *first.  Each word is looked at by `by` neighbouring
+// threads, which count a share of the others.  All threads, between two barriers of the caller's.
+static __device__ __forceinline__ void kth_part(const uint32_t* parts, int k, uint32_t* kth, uint32_t* first) {
+    const int tid = threadIdx.x, count = k <= 32 ? 64 : 128, by = kThreads / count, n = count / 4 / by;
+    const uint32_t part = parts[tid / by];
+    const uint4* share = reinterpret_cast<const uint4*>(parts) + tid % by * n;
+    int larger = 0, not_smaller = 0;
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
         const uint4 other = share[i];
         larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
@@ -342,10 +340,19 @@ static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, in
 #pragma unroll
     for (int o = 1; o < kThreads / 64; o <<= 1)
         if (o < by) both += __shfl_xor_sync(0xffffffffu, both, o);
-    if ((both & 0xffff) < k && k <= both >> 16) sh.bound = unordered(part);      // (equal ones write the same)
+    if ((both & 0xffff) < k && k <= both >> 16) *kth = part;      // (equal ones write the same)
+    if ((both & 0xffff) == 0) *first = part;
+}
+
+// The k-th largest of maxima over all that some threads each have seen: k logits so far are at or above it.
+static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
+    atomicMax(&sh.part_max[threadIdx.x % (k <= 32 ? 64 : 128)], ordered(so_far));      // (what was there is of earlier tiles)
     __syncthreads();
-    *raised = sh.bound > bound;
-    return sh.bound;
+    kth_part(sh.part_max, k, &sh.bound, &sh.highest);
+    __syncthreads();
+    const float now = unordered(sh.bound);
+    *raised = now > bound;
+    return now;
 }
 
 // A chunk of a row: its partial sum, and its k largest keys in descending order.
@@ -358,7 +365,6 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     if (tid == 0) {
         sh.count = 0;
         sh.lost = false;
-        sh.bound = -INFINITY;
     }
     if (tid < 128) sh.part_max[tid] = ordered(-INFINITY);
     __syncthreads();
@@ -569,24 +575,26 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     // ---- everything there is to read, then the beams' sums, eight lanes each
     const Key* keys = p.lists + static_cast<int64_t>(g) * entries;
     const Partial* partials = p.partials + static_cast<int64_t>(g) * lists;
+    Key key[4];
+    const auto load = [&](int e0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) key[u] = e0 + u * kThreads < entries ? __ldcg(keys + e0 + u * kThreads) : 0;
+    };
+    const auto store = [&](int e0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (e0 + u * kThreads < entries) sh.entry[e0 + u * kThreads] = key[u];
+    };
     float ref[kParts], score = 0.f;
     double sum[kParts];
     bool ended = false;
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
         if (i * kThreads + tid < lists) ref[i] = __ldcg(&partials[i * kThreads + tid].ref), sum[i] = __ldcg(&partials[i * kThreads + tid].sum);
+    load(tid);
     if (tid < a.width) {
         score = a.scores[g * a.width + tid];
         ended = a.finished && a.finished[g * a.width + tid];
-    }
-#pragma unroll 1
-    for (int e0 = tid; e0 < entries; e0 += 4 * kThreads) {
-        Key key[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) key[u] = e0 + u * kThreads < entries ? __ldcg(keys + e0 + u * kThreads) : 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (e0 + u * kThreads < entries) sh.entry[e0 + u * kThreads] = key[u];
     }
 #pragma unroll
     for (int i = 0; i < kParts; ++i)
@@ -595,7 +603,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         sh.kind[tid] = !(fabsf(score) < INFINITY) ? 2 : ended;
         sh.score[tid] = score;
     }
-    if (tid == 0) sh.survivors = sh.there = 0, sh.least = 0;
+    if (tid == 0) sh.survivors = sh.there = 0;
     if (tid < 128) sh.front[tid] = 0;
     __syncthreads();
 #pragma unroll 1
@@ -611,6 +619,12 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         for (int o = 4; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         if (w < a.width && (lane & 7) == 0) sh.lse[w] = most + log(total);      // (of a beam that was not read: not used)
     }
+    store(tid);
+#pragma unroll 1
+    for (int e0 = tid + 4 * kThreads; e0 < entries; e0 += 4 * kThreads) {
+        load(e0);
+        store(e0);
+    }
     __syncthreads();
 
     // ---- values as ordered words (0 none), in 64 bits where they are compared, in 32 where they are only bounded
@@ -621,7 +635,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         return sh.kind[w] == 0 && key ? ordered((sh.score[w] + unordered(static_cast<uint32_t>(key >> 32))) - sh.lse[w]) : 0;
     };
     const auto rounded = [](Key v) -> uint32_t { return v ? ordered(static_cast<float>(unordered(v))) : 0u; };
-    // the first of every list, 16 k or 256 together, in 128 shares (neighbours in a list in different ones): nothing below
+    // the first of every list, 16 k or 256 together, in 64 or 128 shares (neighbours in a list in different ones): nothing below
     // the k-th largest of the shares' largest is among the k best
     const int deep = min(k, (max(16 * k, 256) + lists - 1) / lists);
     const float by_deep = 1.f / deep;
@@ -631,23 +645,11 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         const int list = static_cast<int>((i + 0.5f) * by_deep);      // i / deep
         part = max(part, rounded(value(list * k + i - list * deep)));
     }
-    if (kThreads == 128) sh.front[tid] = part;
-    else if (part) atomicMax(&sh.front[tid % 128], part);
+    if (part) atomicMax(&sh.front[tid % (k <= 32 ? 64 : 128)], part);
     __syncthreads();
-    if (tid < 128) {
-        part = sh.front[tid];
-        int larger = 0, not_smaller = 0;
-#pragma unroll 4
-        for (int i = 0; i < 128; i += 4) {
-            const uint4 other = *reinterpret_cast<const uint4*>(&sh.front[i]);
-            larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
-            not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
-        }
-        if (larger < k && k <= not_smaller) sh.least = part;
-        if (larger == 0) sh.top = part;
-    }
+    kth_part(sh.front, k, &sh.bound, &sh.highest);
     __syncthreads();
-    const uint32_t least = max(sh.least, 1u);
+    const uint32_t least = max(sh.bound, 1u);
     // the bound as a logit of each beam, a little lower (what is compared with it is rounded in other places)
     if (tid < a.width) {
         const double logit = unordered(least) - sh.score[tid] + sh.lse[tid];
@@ -673,7 +675,7 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         uint32_t mine[kEntries / kThreads];
 #pragma unroll
         for (int i = 0; i < kEntries / kThreads; ++i) mine[i] = i * kThreads + tid < entries ? rounded(value(i * kThreads + tid)) : 0;
-        const uint32_t bound = static_cast<uint32_t>(kth_largest(k, least, sh.top, sh.hits, [&](const auto& f) {
+        const uint32_t bound = static_cast<uint32_t>(kth_largest(k, least, sh.highest, sh.hits, [&](const auto& f) {
 #pragma unroll
             for (int i = 0; i < kEntries / kThreads; ++i)
                 if (i * kThreads < entries) f(static_cast<Key>(mine[i]));
