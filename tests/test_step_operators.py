@@ -108,6 +108,7 @@ def test_beam_reorder_other_refusals():
     assert L.lib.wuda_beam_reorder(ok, FAKE, None, 3 * FAKE, 1, None, None) == INVALID
     assert L.lib.wuda_beam_reorder(ok, FAKE, 2 * FAKE, 2 * FAKE, 1, None, None) == INVALID and "its own" in message()
     assert L.lib.wuda_beam_reorder(ok, FAKE, 2 * FAKE, FAKE, 1, None, None) == INVALID and "its own" in message()
+    assert L.lib.wuda_beam_reorder(ok, FAKE, 2 * FAKE, 2 * FAKE + 12, 1, None, None) == INVALID and "its own" in message()
 
 
 def test_struct_layouts_match_the_header(tmp_path):

@@ -280,6 +280,10 @@ def test_a_slot_without_a_request_is_refused_and_the_state_has_one_owner():
     assert int(status) == 163 and tables.lengths.tolist()[a] == 1 and tables.out["state_row"].tolist()[1] == -1
     with pytest.raises(wuda.WudaError):
         tables.push()
+    for change in (cache.alloc_request, lambda: cache.free_request(a), lambda: cache.step_begin([a]), lambda: cache.advance(a, 1),
+                   lambda: cache.fork_request(a, 0), lambda: CacheTables(cache, 2)):
+        with pytest.raises(RuntimeError):
+            change()
     tables.pull()
     assert cache.reqs[a]["pos"] == 0
     for call in (tables.pull, lambda: tables.step(torch.zeros(1, dtype=torch.int32, device="cuda"))):

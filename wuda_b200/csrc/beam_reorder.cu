@@ -265,7 +265,9 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
     WUDA_REQUIRE(a.num_pools >= 0 && a.num_pools <= WUDA_BEAM_MAX_POOLS, "num_pools must be in [0, %d]", WUDA_BEAM_MAX_POOLS);
     WUDA_REQUIRE(a.lengths, "lengths must not be NULL");
     WUDA_REQUIRE(groups == 0 || (parents && slots && slots_out), "parents, slots and slots_out must not be NULL");
-    WUDA_REQUIRE(groups == 0 || (slots_out != slots && slots_out != parents), "slots_out must be an array of its own");
+    const int beams = groups * a.width;
+    WUDA_REQUIRE(groups == 0 || ((slots_out + beams <= slots || slots + beams <= slots_out) && (slots_out + beams <= parents || parents + beams <= slots_out)),
+                 "slots_out must be an array of its own");
     Params p = {};
     p.a = a;
     p.per_group = Divisor(a.width);
@@ -305,7 +307,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
     if (groups == 0) return WUDA_OK;
     DeviceInfo dev;
     if (const int st = current_device_info(&dev)) return st;
-    const int rows = groups * a.width;
+    const int rows = beams;
     const size_t smem = shared_bytes(rows, a.capacity);
     if (smem > 48 * 1024 - 1024)
         WUDA_CUDA(cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

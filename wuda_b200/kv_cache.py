@@ -86,6 +86,7 @@ class KVCacheManager:
         self._free_slots = list(range(capacity - 1, -1, -1))
         self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables, "shared": tokens in shared pages}
         self._owners = {"cmp": {}, "idx": {}}      # page -> requests that hold it, where they are more than one
+        self.on_device = False  # step tables on the device (step_tables.CacheTables) have the requests' state: nothing changes here
 
     # ---- slot lifecycle: a new or reused slot starts with kv = 0, score = -inf
     def _reset_state(self, slot):
@@ -93,7 +94,12 @@ class KVCacheManager:
             state[slot, :, :half] = 0.0
             state[slot, :, half:] = NEG_INF
 
+    def _need_state(self):
+        if self.on_device:
+            raise RuntimeError("the requests' state is in step tables on the device: pull() it first")
+
     def alloc_request(self):
+        self._need_state()
         slot = self._free_slots.pop()
         self._reset_state(slot)
         swa = self._pools["swa"]
@@ -105,6 +111,7 @@ class KVCacheManager:
         """Bookkeeping of a prefill of `tokens` tokens (not in the reference's manager): moves the
         request's position forward and takes the pages its compressed entries occupy, without
         producing per-token destinations.  The caches themselves are filled by whoever prefills."""
+        self._need_state()
         req = self.reqs[slot]
         req["pos"] += int(tokens)
         entries = (req["pos"] + 1) // RATIO
@@ -113,6 +120,7 @@ class KVCacheManager:
                 self._pools[name].entry(req[name], entries - 1)
 
     def free_request(self, slot):
+        self._need_state()
         req = self.reqs.pop(slot)
         for name in ("swa", "cmp", "idx"):
             self._pools[name].give_back(self._given_up(name, req[name]))
@@ -138,6 +146,7 @@ class KVCacheManager:
         """`copies` new requests that continue request `slot` (the beams of a prompt; not in the reference's manager).  Returns
         their slots.  All of them, the request included, share its filled compressed pages; state rings, window pages and
         the compressed page that is being filled are copied.  A request that shares pages already is not forked again."""
+        self._need_state()
         req = self.reqs[slot]
         if req.get("shared"):
             raise ValueError("request %d shares its pages already" % slot)
@@ -167,6 +176,7 @@ class KVCacheManager:
 
     # ---- one decode step: positions, state rows and cache destinations of every request
     def step_begin(self, slots):
+        self._need_state()
         pos, idx_dst, cmp_dst, swa_dst = [], [], [], []
         swa = self._pools["swa"]
         for s in slots:

@@ -98,8 +98,6 @@ class AttentionHalfLayer:
 
     def prepare(self, slots):
         """Host side of a step: positions, destinations, page tables, window entries (device copies only)."""
-        if self.tables is not None and self.tables.on_device:
-            raise _lib.WudaError(1, "the cache's step tables are on the device: prepare_on_device(), or pull() them first")
         st = self.stage.prepare(slots)
         m = len(slots)
         pos = st["pos"].tolist()

@@ -138,7 +138,7 @@ class CacheTables(StepTables):
         epb = cache.entries_per_block
         pages = {name: cache._pools[name].data.size(0) for name in ("idx", "cmp")}
         self.shared_lengths = i32(cache.capacity)
-        self.on_device = False      # who has the state: the device, from a push() to the next pull(), or the manager
+        self._pushed = False        # who has the state: these tables, from a push() to the next pull(), or the manager
         super().__init__(i32(cache.capacity), i32(cache.capacity, cache.max_pages), i32(cache.capacity, cache.max_pages),
                          i32(cache.capacity, -(-WIN // epb["swa"])), i32(pages["idx"]), i32(pages["cmp"]), i32(2),
                          max_rows=max_rows, max_tokens=max_tokens, idx_entries_per_block=epb["idx"],
@@ -148,9 +148,9 @@ class CacheTables(StepTables):
 
     def push(self):
         """The manager's state to the device, on the current stream."""
-        if self.on_device:
-            raise _lib.WudaError(1, "the state is on the device: pull() it before the manager changes anything")
         cache = self.cache
+        if cache.on_device:
+            raise _lib.WudaError(1, "the state is on the device: pull() it before the manager changes anything")
         lengths, shared = [-1] * cache.capacity, [0] * cache.capacity      # (a slot without a request is refused)
         tables = {name: torch.zeros(tuple(t.shape), dtype=torch.int32)
                   for name, t in (("idx", self.idx_table), ("cmp", self.cmp_table), ("swa", self.swa_table))}
@@ -168,12 +168,12 @@ class CacheTables(StepTables):
         self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
         self.shared_lengths.copy_(torch.tensor(shared, dtype=torch.int32))
         self.free_counts.copy_(torch.tensor([len(cache._pools[name]._free) for name in ("idx", "cmp")], dtype=torch.int32))
-        self.on_device = True
+        cache.on_device = self._pushed = True
 
     def pull(self):
         """The device's state back into the manager; waits for the current stream.  Captured steps are not replayed until the
         next push()."""
-        if not self.on_device:
+        if not self._pushed:
             raise _lib.WudaError(1, "the manager has the state already")
         cache = self.cache
         lengths, counts = self.lengths.tolist(), self.free_counts.tolist()
@@ -184,10 +184,10 @@ class CacheTables(StepTables):
                 req[name] = rows[slot, :-(-(lengths[slot] // RATIO) // epb)].tolist()
         for slot, req in cache.reqs.items():
             req["pos"] = lengths[slot] - 1
-        self.on_device = False
+        cache.on_device = self._pushed = False
 
     def step(self, slots, new_tokens=None):
-        if not self.on_device:
+        if not self._pushed:
             raise _lib.WudaError(1, "the cache manager has the state: push() it first")
         return super().step(slots, new_tokens)
 
