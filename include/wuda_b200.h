@@ -1097,7 +1097,8 @@ int wuda_step_tables(const wuda_step_tables_args* args, const int32_t* slots, co
  * in descending order; equal values are resolved towards the lower beam, then the lower token.  The comparison is that of
  * (score + logit) - log sum in 64 bits (within a beam: of the logits); sums of exponentials are held in 32 bits per thread and 64 across threads.
  * A logit that is not finite (a masked token) takes no part, a score that is not finite ends its beam: it has no
- * continuation.  A finished beam has one, (scores[g, w], eos_token); the logits of either are not read.
+ * continuation.  A finished beam has one, (scores[g, w], eos_token).  What the logits of either hold has no effect (a finished
+ * beam's are not read).
  * Where a group has fewer than k continuations, the rest is (-inf, parent -1, token -1).
  *   finished_out[g, j] = the parent is finished, or the token is eos_token
  *

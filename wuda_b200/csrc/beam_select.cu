@@ -362,12 +362,6 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     const wuda_beam_select_args& a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, k = a.k;
     const int c0 = number * p.chunk_vectors * kVec, end = min(a.vocab, c0 + p.chunk_vectors * kVec);
-    if (tid == 0) {
-        sh.count = 0;
-        sh.lost = false;
-    }
-    if (tid < 128) sh.part_max[tid] = ordered(-INFINITY);
-    __syncthreads();
     constexpr int kTile = kThreads * kVectors * kVec;
     const int tiles = (end - c0 + kTile - 1) / kTile, whole = (end - c0) / kTile;
     // A row's last, partial tile is spread over the threads, a vector each first, so that there are maxima of many parts of it.  In a
@@ -416,6 +410,12 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     if (a.finished && a.finished[row_number]) return;
     fetch(0);      // on its way while the score is
     if (!(fabsf(a.scores[row_number]) < INFINITY)) return;
+    if (tid == 0) {
+        sh.count = 0;
+        sh.lost = false;
+    }
+    if (tid < 128) sh.part_max[tid] = ordered(-INFINITY);
+    __syncthreads();
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
     int noted = 0;        // of the warp's vectors
@@ -759,8 +759,8 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
     const wuda_beam_select_args& a = p.a;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
-    const int number = blockIdx.x % p.chunks, row = blockIdx.x / p.chunks, g = row / a.width;
-    const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + (row - g * a.width) * a.beam_stride;
+    const int number = blockIdx.x, g = blockIdx.z, row = g * a.width + blockIdx.y;
+    const T* x = static_cast<const T*>(a.logits) + g * a.group_stride + blockIdx.y * a.beam_stride;
     B::template chunk<T, ALIGNED>(sh, p, x, row, number);
     __threadfence();
     __syncthreads();
@@ -854,7 +854,7 @@ extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream)
          {beam_select_kernel<__nv_bfloat16, 512, false>, beam_select_kernel<__half, 512, false>, beam_select_kernel<float, 512, false>}},
         {{beam_select_kernel<__nv_bfloat16, 128, true>, beam_select_kernel<__half, 128, true>, beam_select_kernel<float, 128, true>},
          {beam_select_kernel<__nv_bfloat16, 512, true>, beam_select_kernel<__half, 512, true>, beam_select_kernel<float, 512, true>}}};
-    WUDA_CUDA(launch_pdl(kernels[aligned][c.threads == 512][a.logits_type], dim3(static_cast<unsigned>(parts)), dim3(c.threads), 0,
+    WUDA_CUDA(launch_pdl(kernels[aligned][c.threads == 512][a.logits_type], dim3(c.chunks, a.width, a.groups), dim3(c.threads), 0,
                          static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }

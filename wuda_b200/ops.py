@@ -232,7 +232,7 @@ def beam_select(logits, scores, k=None, *, finished=None, eos_token=None):
       finished bool  [groups, k]  the parent is finished, or the token is eos_token
     Equal values go to the lower beam, then the lower token.  Logits that are not finite take no part (masked tokens), a
     beam whose score is not finite has no continuation, a finished beam (finished bool [groups, width], with an
-    eos_token) only itself with eos_token; the logits of both are not read.  Where fewer than k continuations are left, the rest is
+    eos_token) only itself with eos_token, whatever their logits hold.  Where fewer than k continuations are left, the rest is
     (-inf, -1, -1, False).  groups <= 256, width <= 32, k <= 64."""
     done = _fast.beam_select(logits, scores, k, finished, eos_token, _beam_scratch._streams, FLAG_BYTES)
     if done is not None:
