@@ -64,35 +64,43 @@ __device__ __forceinline__ int pieces_of(const Params& p, int pool, const Span& 
     return (s.pages - 1 - s.first_page) * static_cast<int>(p.per_page[pool].by) + ((last + (1 << p.piece_shift[pool]) - 1) >> p.piece_shift[pool]);
 }
 
-// What one piece copies: up to two runs of bytes (multiples of 4), the second behind the first only in its number of units.
+// What one piece copies: up to two runs of units of 16 bytes, or of 4 where not everything lies on 16.
 struct Piece {
     const uint8_t* src[2];
     uint8_t* dst[2];
-    int bytes[2];
+    int units[2];
+    bool wide;
+    __device__ __forceinline__ void in_units() {      // of bytes
+        uintptr_t bits = units[0] | units[1];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) bits |= reinterpret_cast<uintptr_t>(src[k]) | reinterpret_cast<uintptr_t>(dst[k]);
+        wide = (bits & 15) == 0;
+        units[0] >>= wide ? 4 : 2;
+        units[1] >>= wide ? 4 : 2;
+    }
 };
 
-// By all threads of the block: four units in flight per thread, loads first.  A unit is 16 bytes where everything lies on 16, else 4.
+// By all threads of the block: four units in flight per thread, loads first.  Addresses by constant steps from two pointers: an index
+// into either run for every unit takes five times the instructions.
 template <typename Unit>
-__device__ __forceinline__ void copy_units(const Piece& c, int n0, int n) {
-    for (int i0 = 0; i0 < n; i0 += kUnroll * kThreads) {
+__device__ __forceinline__ void copy_units(const Piece& c) {
+    const int tid = threadIdx.x, n1 = c.units[1];
+    const Unit* src = reinterpret_cast<const Unit*>(c.src[0]) + tid;
+    Unit* dst = reinterpret_cast<Unit*>(c.dst[0]) + tid;
+    for (int rest = c.units[0] - tid; rest > 0; rest -= kUnroll * kThreads) {
         Unit v[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = i0 + u * kThreads + threadIdx.x;
-            if (i < n) v[u] = i < n0 ? __ldcs(reinterpret_cast<const Unit*>(c.src[0]) + i) : __ldcs(reinterpret_cast<const Unit*>(c.src[1]) + i - n0);
-        }
+        for (int u = 0; u < kUnroll; ++u)
+            if (u * kThreads < rest) v[u] = __ldcs(src + u * kThreads);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = i0 + u * kThreads + threadIdx.x;
-            if (i < n) *(i < n0 ? reinterpret_cast<Unit*>(c.dst[0]) + i : reinterpret_cast<Unit*>(c.dst[1]) + i - n0) = v[u];
-        }
+        for (int u = 0; u < kUnroll; ++u)
+            if (u * kThreads < rest) __stcs(dst + u * kThreads, v[u]);
+        src += kUnroll * kThreads;
+        dst += kUnroll * kThreads;
     }
-}
-__device__ __forceinline__ void copy_piece(const Piece& c) {
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(c.src[0]) | reinterpret_cast<uintptr_t>(c.dst[0]) | reinterpret_cast<uintptr_t>(c.src[1]) |
-                           reinterpret_cast<uintptr_t>(c.dst[1]) | c.bytes[0] | c.bytes[1];
-    if (bits & 15) copy_units<uint32_t>(c, c.bytes[0] / 4, (c.bytes[0] + c.bytes[1]) / 4);
-    else copy_units<uint4>(c, c.bytes[0] / 16, (c.bytes[0] + c.bytes[1]) / 16);
+    // the second run from the last threads, which have least of the first
+    for (int i = kThreads - 1 - tid; i < n1; i += kThreads)
+        reinterpret_cast<Unit*>(c.dst[1])[i] = __ldcs(reinterpret_cast<const Unit*>(c.src[1]) + i);
 }
 
 __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const __grid_constant__ Params p) {
@@ -202,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
             const int64_t bytes = a.states[i].row_bytes, at = static_cast<int64_t>(piece - p.state_first[i]) * kPieceBytes;
             uint8_t* data = static_cast<uint8_t*>(a.states[i].data);
             c.src[0] = data + src * bytes + at, c.dst[0] = data + dst * bytes + at;
-            c.bytes[0] = static_cast<int>(min(static_cast<int64_t>(kPieceBytes), bytes - at));
+            c.units[0] = static_cast<int>(min(static_cast<int64_t>(kPieceBytes), bytes - at));
             return c;
         }
         piece -= p.state_pieces;
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
                 const int64_t size = pool.segment_bytes[k], at = offset + e0 * size;
                 c.src[k] = static_cast<const uint8_t*>(pool.data) + from * pool.stride_bytes + at;
                 c.dst[k] = static_cast<uint8_t*>(pool.data) + to * pool.stride_bytes + at;
-                c.bytes[k] = static_cast<int>((e1 - e0) * size);
+                c.units[k] = static_cast<int>((e1 - e0) * size);
                 offset += pool.entries_per_block * size;
             }
             return c;
@@ -241,9 +249,16 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
     for (int64_t unit = blockIdx.x; unit < total[0]; unit += static_cast<int64_t>(kBatch) * gridDim.x) {
         const int64_t last = total[0] - 1 - unit;
         const int n = static_cast<int>(min(last / gridDim.x + 1, static_cast<int64_t>(kBatch)));
-        if (tid < n) pieces[tid] = piece_of(static_cast<int>(unit + static_cast<int64_t>(tid) * gridDim.x));
+        if (tid < n) {
+            Piece c = piece_of(static_cast<int>(unit + static_cast<int64_t>(tid) * gridDim.x));
+            c.in_units();
+            pieces[tid] = c;
+        }
         __syncthreads();
-        for (int i = 0; i < n; ++i) copy_piece(pieces[i]);
+        for (int i = 0; i < n; ++i) {
+            if (pieces[i].wide) copy_units<uint4>(pieces[i]);
+            else copy_units<uint32_t>(pieces[i]);
+        }
         __syncthreads();
     }
 }
