@@ -1141,7 +1141,7 @@ int wuda_beam_select(const wuda_beam_select_args* args, void* stream);
  * negative lengths, or of more pages than the table has, is not made and its beam gets slot -1 (WUDA_DEV_BAD_LENGTH); a page
  * outside the pool is not copied (WUDA_DEV_BAD_PAGE_INDEX).
  *
- * width <= 32, groups * width <= 4096, capacity <= 16384.  slots_out must not be slots.
+ * width <= 32, groups * width <= 4096, capacity <= 16384, an entry at most 16 MB.  slots_out overlaps neither slots nor parents.
  */
 #define WUDA_BEAM_MAX_STATES 8
 #define WUDA_BEAM_MAX_POOLS 4

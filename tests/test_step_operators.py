@@ -101,6 +101,14 @@ def test_beam_reorder_refusals(args, groups, word):
     assert st == INVALID and word in message(), message()
 
 
+@pytest.mark.parametrize("pool, word", [
+    (dict(entries_per_block=4, segment_bytes=(1 << 30, 1 << 30), stride_bytes=1 << 33), "16 MB"),
+    (dict(entries_per_block=1 << 30, table_width=1 << 30, segment_bytes=(16, 0), stride_bytes=1 << 34), "pieces")])
+def test_beam_reorder_refuses_what_does_not_fit_its_numbers(pool, word):
+    st = L.lib.wuda_beam_reorder(ctypes.byref(reorder(pools=(pool,) * 4)), FAKE, 2 * FAKE, 3 * FAKE, 1024, None, None)
+    assert st == INVALID and word in message(), message()
+
+
 def test_beam_reorder_other_refusals():
     ok = ctypes.byref(reorder())
     assert L.lib.wuda_beam_reorder(None, FAKE, FAKE, FAKE, 1, None, None) == INVALID

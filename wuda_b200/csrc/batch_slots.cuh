@@ -1,5 +1,8 @@
 // The request slots of a batch in shared memory: which rows have one, and which row has it first.  Every CTA of a kernel finds
 // that out for itself (a few hundred cycles beside the loads that it waits for anyway), so that no launch is needed in front.
+//
+// What an earlier kernel may have written is read through L2 (__ldcg) here and in the kernels that include this: they start while
+// that kernel runs, and a line in their SM's L1 may be older than its writes.
 #pragma once
 #include <climits>
 
@@ -41,12 +44,13 @@ __device__ __forceinline__ void report(int32_t* status, int code) {
     if (status) atomicCAS(status, 0, code);
 }
 
-// slot[b] = slots[b], or -1 where it is outside [0, capacity) or an earlier row has it.  `first`: capacity words, whatever they
-// hold.  All threads of the block; the rows of a thread are [b0, b1).  Ends behind a barrier.
-__device__ __forceinline__ void load_slots(const int32_t* __restrict__ slots, int b0, int b1, int capacity, int* slot, int* first,
-                                           int32_t* status) {
+// slot[b] = given(b), or -1 where it is outside [0, capacity) or an earlier row has it.  `first`: capacity words, whatever they
+// hold.  All threads of the block; the rows of a thread are [b0, b1), and what it leaves of them only that thread may read before the
+// next barrier.
+template <typename Given>
+__device__ __forceinline__ void take_slots(const Given& given, int b0, int b1, int capacity, int* slot, int* first, int32_t* status) {
     for (int b = b0; b < b1; ++b) {
-        const int s = slots[b];
+        const int s = given(b);
         const bool inside = s >= 0 && s < capacity;
         if (!inside && s != -1) report(status, WUDA_DEV_BAD_SLOT);
         slot[b] = inside ? s : -1;

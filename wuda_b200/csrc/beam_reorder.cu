@@ -91,7 +91,7 @@ __device__ __forceinline__ void copy_units(const Piece& c) {
         Unit v[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-            if (u * kThreads < rest) v[u] = __ldcs(src + u * kThreads);
+            if (u * kThreads < rest) v[u] = __ldcg(src + u * kThreads);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
             if (u * kThreads < rest) __stcs(dst + u * kThreads, v[u]);
@@ -100,7 +100,7 @@ __device__ __forceinline__ void copy_units(const Piece& c) {
     }
     // the second run from the last threads, which have least of the first
     for (int i = kThreads - 1 - tid; i < n1; i += kThreads)
-        reinterpret_cast<Unit*>(c.dst[1])[i] = __ldcs(reinterpret_cast<const Unit*>(c.src[1]) + i);
+        reinterpret_cast<Unit*>(c.dst[1])[i] = __ldcg(reinterpret_cast<const Unit*>(c.src[1]) + i);
 }
 
 __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const __grid_constant__ Params p) {
@@ -117,20 +117,20 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
     int* donor = source + rows;      // ... and the beam that has it
     int* own = donor + rows;         // its slot
     int* begin = own + rows;         // the number of its first piece
-    int* first = begin + rows;       // (load_slots)
+    int* first = begin + rows;       // (take_slots)
     int32_t* status = blockIdx.x == 0 ? p.status : nullptr;
     pdl_launch_dependents();
     pdl_wait();   // nothing of global memory is touched before the kernel ahead has finished
     const int per = (rows + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, rows), b1 = min(b0 + per, rows);
     for (int b = b0; b < b1; ++b) {
-        parents[b] = p.parents[b];
-        const int s = p.slots[b];
+        parents[b] = __ldcg(p.parents + b);
+        const int s = slot[b] = __ldcg(p.slots + b);
         const bool inside = s >= 0 && s < a.capacity;
-        length[b] = inside ? a.lengths[s] : -1;
-        common[b] = inside && a.shared_lengths ? a.shared_lengths[s] : 0;
+        length[b] = inside ? __ldcg(a.lengths + s) : -1;
+        common[b] = inside && a.shared_lengths ? __ldcg(a.shared_lengths + s) : 0;
     }
-    load_slots(p.slots, b0, b1, a.capacity, slot, first, status);
+    take_slots([&](int b) { return slot[b]; }, b0, b1, a.capacity, slot, first, status);
     __syncthreads();
 
     // ---- new slots and forks, and how much each fork copies: a lane per new beam, as many whole groups to a warp as fit
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
             const int of = static_cast<int>(p.per_page[i].quotient(piece)), page = s.first_page + of;
             const int e0 = (piece - of * static_cast<int>(p.per_page[i].by)) << p.piece_shift[i];
             const int e1 = min(min(e0 + (1 << p.piece_shift[i]), pool.entries_per_block), s.entries - page * pool.entries_per_block);
-            const int from = pool.table[static_cast<int64_t>(src) * pool.table_width + page];
-            const int to = pool.table[static_cast<int64_t>(dst) * pool.table_width + page];
+            const int from = __ldcg(pool.table + static_cast<int64_t>(src) * pool.table_width + page);
+            const int to = __ldcg(pool.table + static_cast<int64_t>(dst) * pool.table_width + page);
             if (from < 0 || from >= pool.num_blocks || to < 0 || to >= pool.num_blocks) {
                 report(p.status, WUDA_DEV_BAD_PAGE_INDEX);
                 return c;
@@ -302,6 +302,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
                      "pool %d: sizes must be positive", i);
         WUDA_REQUIRE(q.segment_bytes[0] > 0 && q.segment_bytes[0] % 4 == 0 && q.segment_bytes[1] >= 0 && q.segment_bytes[1] % 4 == 0,
                      "pool %d: segments must be multiples of 4 bytes", i);
+        WUDA_REQUIRE(record <= 1 << 24, "pool %d: an entry of more than 16 MB", i);
         WUDA_REQUIRE(q.segment_bytes[1] == 0 || static_cast<int64_t>(q.entries_per_block) * q.segment_bytes[0] % 16 == 0,
                      "pool %d: the second segment must start on 16 bytes", i);
         WUDA_REQUIRE(q.stride_bytes >= q.entries_per_block * record, "pool %d: a page does not hold its entries", i);
@@ -314,7 +315,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
         // the table's pages bound the pieces of a fork
         pieces += static_cast<int64_t>(q.table_width) * p.per_page[i].by;
     }
-    WUDA_REQUIRE(pieces * groups * a.width < INT_MAX, "a reordering of more than 2^31 pieces");
+    WUDA_REQUIRE(pieces < INT_MAX && pieces * groups * a.width < INT_MAX, "a reordering of more than 2^31 pieces");
     for (int i = 0; i < a.num_states; ++i) {
         p.state_pieces += static_cast<int>((a.states[i].row_bytes + kPieceBytes - 1) / kPieceBytes);
         p.state_first[i + 1] = p.state_pieces;

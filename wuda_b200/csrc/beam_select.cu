@@ -105,10 +105,11 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return c;
 }
 
-// ---- a vector: 16 bytes of a row as four words
+// ---- a vector: 16 bytes of a row as four words, through L2: the kernel starts while the one that writes the logits runs, and a line
+// in its SM's L1 may be older than them
 __device__ __forceinline__ uint4 load16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 
@@ -120,9 +121,9 @@ __device__ __noinline__ uint4 load_elements(const T* row, int at, int vocab) {
     for (int i = 0; i < Type<T>::kVec; ++i) {
         if (at + i < 0 || at + i >= vocab) continue;
         if constexpr (sizeof(T) == 4) {
-            w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
+            w[i] = __ldcg(reinterpret_cast<const uint32_t*>(row) + at + i);
         } else {
-            const uint32_t x = reinterpret_cast<const uint16_t*>(row)[at + i];
+            const uint32_t x = __ldcg(reinterpret_cast<const uint16_t*>(row) + at + i);
             w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (x << 16) : (w[i / 2] & 0xffff0000u) | x;
         }
     }
@@ -407,9 +408,9 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
             for (int i = 0; i < 4; ++i) w[4 * u + i] = __funnelshift_r(x[SKIP + i], x[SKIP + i + 1], bits);
         }
     };
-    if (a.finished && a.finished[row_number]) return;
+    if (a.finished && __ldcg(a.finished + row_number)) return;
     fetch(0);      // on its way while the score is
-    if (!(fabsf(a.scores[row_number]) < INFINITY)) return;
+    if (!(fabsf(__ldcg(a.scores + row_number)) < INFINITY)) return;
     if (tid == 0) {
         sh.count = 0;
         sh.lost = false;
@@ -593,8 +594,8 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
         if (i * kThreads + tid < lists) ref[i] = __ldcg(&partials[i * kThreads + tid].ref), sum[i] = __ldcg(&partials[i * kThreads + tid].sum);
     load(tid);
     if (tid < a.width) {
-        score = a.scores[g * a.width + tid];
-        ended = a.finished && a.finished[g * a.width + tid];
+        score = __ldcg(a.scores + g * a.width + tid);
+        ended = a.finished && __ldcg(a.finished + g * a.width + tid);
     }
 #pragma unroll
     for (int i = 0; i < kParts; ++i)

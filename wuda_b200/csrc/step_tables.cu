@@ -34,14 +34,15 @@ struct Rows {
     int* cmp_first;
     int* idx_need;    // and that it takes itself
     int* cmp_need;
+    int* count;       // tokens
     int* start;       // rows + 1
-    int* first;       // (load_slots)
+    int* first;       // (take_slots)
     __device__ Rows(int* mem, int rows) {
         slot = mem, old_len = slot + rows, new_len = old_len + rows, idx_first = new_len + rows, cmp_first = idx_first + rows;
-        idx_need = cmp_first + rows, cmp_need = idx_need + rows, start = cmp_need + rows, first = start + rows + 1;
+        idx_need = cmp_first + rows, cmp_need = idx_need + rows, count = cmp_need + rows, start = count + rows, first = start + rows + 1;
     }
 };
-inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (8ull * rows + 1 + capacity); }
+inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (9ull * rows + 1 + capacity); }
 
 __device__ __forceinline__ int pages_of(const Params& p, uint32_t tokens, const Divisor& epb) {
     return static_cast<int>(epb.quotient_up(p.ratio.quotient(tokens)));
@@ -58,7 +59,7 @@ struct PoolView {
     const int32_t* table;   // the slot's row
     const int32_t* free;
     int held, top;          // page `held` is free[top], the next one free[top - 1]
-    __device__ int operator()(int page) const { return page < held ? table[page] : free[top - (page - held)]; }
+    __device__ int operator()(int page) const { return __ldcg(page < held ? table + page : free + (top - (page - held))); }
 };
 
 // entry `entry` of a request, in page `page` of it, as an entry of the pool
@@ -69,7 +70,7 @@ __device__ __forceinline__ int64_t entry_of(int pool_page, const Divisor& epb, u
 __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_constant__ Params p) {
     extern __shared__ int mem[];
     __shared__ int scan[3 * 33];
-    __shared__ int taken[2];
+    __shared__ int taken[2], stacks[2];
     __shared__ bool last;
     const wuda_step_tables_args& a = p.a;
     const int rows = p.rows, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -81,18 +82,21 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_cons
     // ---- the rows
     const int per = (rows + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, rows), b1 = min(b0 + per, rows);
-    load_slots(p.slots, b0, b1, a.capacity, r.slot, r.first, status);
-    const int free_idx = cut_count(a.free_counts[0], a.idx_free_capacity, status);
-    const int free_cmp = cut_count(a.free_counts[1], a.cmp_free_capacity, status);
+    // (one thread of a CTA reads the counts: all of them, of all CTAs, would queue for one address of L2)
+    if (tid == 0) stacks[0] = __ldcg(a.free_counts), stacks[1] = __ldcg(a.free_counts + 1);
+    take_slots([&](int b) { return __ldcg(p.slots + b); }, b0, b1, a.capacity, r.slot, r.first, status);
+    const int free_idx = cut_count(stacks[0], a.idx_free_capacity, tid == 0 ? status : nullptr);
+    const int free_cmp = cut_count(stacks[1], a.cmp_free_capacity, tid == 0 ? status : nullptr);
     int sum[3] = {0, 0, 0}, total[3];      // tokens, pages of both pools
     for (int b = b0; b < b1; ++b) {
-        const int n = p.new_tokens ? p.new_tokens[b] : 1;
+        const int n = p.new_tokens ? __ldcg(p.new_tokens + b) : 1;
         const int counted = min(max(n, 0), a.max_tokens + 1);
         r.start[b] = sum[0];
+        r.count[b] = n;
         sum[0] += counted;
         const int slot = r.slot[b];
         if (slot < 0) continue;
-        const int old = a.lengths[slot];
+        const int old = __ldcg(a.lengths + slot);
         const int64_t now = static_cast<int64_t>(old) + n;
         const bool counts = old >= 0 && n >= 0 && now <= INT_MAX;
         const int idx_pages = counts ? pages_of(p, static_cast<uint32_t>(now), p.idx_epb) : 0;
@@ -118,7 +122,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_cons
     // Rows that would reach beyond the buffers or the stacks.  Their needs are in the sums of the rows behind them, which is the rule:
     // of the rows that need pages none behind the first that finds too few is served.  (Tokens beyond the buffers are a suffix, too.)
     for (int b = b0; b < b1; ++b) {
-        const int n = max(p.new_tokens ? p.new_tokens[b] : 1, 0);
+        const int n = max(r.count[b], 0);
         const int begin = r.start[b] + sum[0];
         r.start[b] = min(begin, a.max_tokens);
         if (r.slot[b] < 0) continue;
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_cons
     }
     if (mine) {
         if (a.lengths_out != a.lengths) {
-            for (int s = tid; s < a.capacity; s += kThreads) a.lengths_out[s] = a.lengths[s];
+            for (int s = tid; s < a.capacity; s += kThreads) a.lengths_out[s] = __ldcg(a.lengths + s);
             __syncthreads();
         }
         for (int b = b0; b < b1; ++b)
@@ -202,9 +206,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_cons
             const int slot = r.slot[b], now = slot >= 0 ? r.new_len[b] : 0;
             const int valid = min(now, a.window);
             const int32_t* pages = a.swa_table + static_cast<int64_t>(max(slot, 0)) * window_pages;
+            const int only = window_pages == 1 ? __ldcg(pages) : 0;
             for (int i = lane; i < a.window; i += 32) {
                 const uint32_t ring = i < valid ? p.window.rest(now - valid + i) : 0, page = p.swa_epb.quotient(ring);
-                a.swa_indices[static_cast<int64_t>(b) * a.window + i] = i < valid ? static_cast<int>((pages[page] - page) * p.swa_epb.by + ring) : -1;
+                a.swa_indices[static_cast<int64_t>(b) * a.window + i] = i < valid ? static_cast<int>(((window_pages == 1 ? only : __ldcg(pages + page)) - page) * p.swa_epb.by + ring) : -1;
             }
             if (lane == 0) {
                 const int entries = static_cast<int>(p.ratio.quotient(now));
@@ -228,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(const __grid_cons
                 if (pos >= now - a.ring_entries) state = static_cast<int64_t>(slot) * a.ring_entries + p.ring.rest(pos);
                 if (pos >= now - a.window) {
                     const uint32_t ring = p.window.rest(pos), page = p.swa_epb.quotient(ring);
-                    swa = entry_of(a.swa_table[static_cast<int64_t>(slot) * window_pages + page], p.swa_epb, page, ring);
+                    swa = entry_of(__ldcg(a.swa_table + static_cast<int64_t>(slot) * window_pages + page), p.swa_epb, page, ring);
                 }
                 const uint32_t done = p.ratio.quotient(pos + 1u);
                 if (done * p.ratio.by == pos + 1u) {
