@@ -60,6 +60,45 @@ def test_steps_prepared_on_the_device_give_the_host_prepared_bits(native, fp4):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+def test_graphs_of_both_ways_of_preparing_live_side_by_side():
+    """A graph captured before the layer had tables on the device replays the host's steps and, later, the device's: the same
+    buffers.  One that prepares its own steps is refused while the cache manager has the state, and with too few slots."""
+    layer, slots, x = build_random_layer(3, 250, seed=31, **SMALL)
+    twin, twin_slots, _ = build_random_layer(3, 250, seed=31, **SMALL)
+    layer.prepare(slots)
+    graph = layer.capture(x, 3)
+    outs = []
+
+    def compare(out):
+        twin.prepare(twin_slots)
+        outs.append(out)
+        assert torch.equal(out, twin.launch(x, 3))
+
+    compare(layer.replay().clone())
+    dev = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    tables = layer.device_tables()
+    for _ in range(3):
+        layer.prepare_on_device(dev)
+        graph.replay()
+        compare(layer._graph_out.clone())
+    with pytest.raises(ValueError):
+        layer.capture(x, 3, slots=dev[:2])
+    layer.capture(x, 3, slots=dev)
+    compare(layer.replay().clone())
+    tables.pull()
+    with pytest.raises(RuntimeError):
+        layer.replay()
+    layer.prepare(slots)
+    graph.replay()
+    compare(layer.out[:3].clone())
+    tables.push()
+    compare(layer.replay().clone())
+    layer.check_status()
+    assert len({tuple(o.view(torch.int16).flatten()[:4096].tolist()) for o in outs}) == len(outs)
+    for a, b in zip(pools_of(layer.attn.cache), pools_of(twin.attn.cache)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 class Head:
     """A stand-in for what lies around the one layer: an embedding and an output projection over a small vocabulary."""
 

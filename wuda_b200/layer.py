@@ -73,17 +73,17 @@ class AttentionHalfLayer:
         self.swa_len = torch.zeros(max_batch, dtype=torch.int32, device=dev)
         self.cmp_len = torch.zeros(max_batch, dtype=torch.int32, device=dev)
         self.stage.q_raw = self.front_out[:, :csa_weights.q_lora]       # the chain reads the q_lora columns in place
+        self.stage.idx_state_row = self.stage.main_state_row            # one ring geometry: the two rings' rows are the same
         self.status = self.stage.status
         self.out = None
         self.tables = None
         self._graph, self._graph_m, self._graph_x = None, 0, None
 
     def device_tables(self):
-        """The cache's step tables on the device, filling this layer's step buffers (made by the first call, which takes over the
-        cache manager's present state; later changes there need tables.push())."""
+        """The cache's step tables on the device, filling this layer's step buffers.  The first call takes the state over from the
+        cache manager, which then refuses prepare() and every other change until tables.pull(); push() takes it over again."""
         if self.tables is None:
             st = self.stage
-            st.idx_state_row = st.main_state_row       # (one ring geometry: the two rings' rows are the same)
             self.tables = CacheTables(
                 self.cache, self.max_batch, topk=self.topk, status_word=self.status,
                 out=dict(pos=st.pos, q_pos=st.q_pos, state_row=st.main_state_row, idx_dst=st.idx_dst, cmp_dst=st.cmp_dst,
@@ -178,7 +178,7 @@ class DecoderLayer:
         self.hidden = hidden
         self.out = torch.empty(max_batch, 4, hidden, dtype=torch.bfloat16, device=dev)
         self.route_indices = None
-        self._graph = None
+        self._graph = self._graph_slots = None
         if native:
             self._init_native(dev)
         else:
@@ -308,24 +308,28 @@ class DecoderLayer:
         their calls on the device.  With slots (int32 [m] on the device) the graph prepares its step itself
         (prepare_on_device), so that every replay is the next token; the eager pass is taken back."""
         if slots is not None:
+            if slots.numel() != m:
+                raise ValueError("slots must be one for each of the %d rows" % m)
             tables = self.device_tables()
             before = tables.lengths.clone(), tables.free_counts.clone()
             self.prepare_on_device(slots)
         self.launch(hidden_states, m)
-        torch.cuda.synchronize()
-        self.check_status()
         if slots is not None:      # (the pages it took are the ones that the first replay takes, and what it wrote is written again)
             tables.lengths.copy_(before[0])
             tables.free_counts.copy_(before[1])
+        torch.cuda.synchronize()
+        self.check_status()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             if slots is not None:
                 self.prepare_on_device(slots)
             out = self.launch(hidden_states, m)
-        self._graph, self._graph_out = graph, out
+        self._graph, self._graph_out, self._graph_slots = graph, out, slots
         return graph
 
     def replay(self):
+        if self._graph_slots is not None and not self.attn.cache.on_device:
+            raise RuntimeError("the graph prepares its steps from the device's state: push() it first")
         self._graph.replay()
         return self._graph_out
 
