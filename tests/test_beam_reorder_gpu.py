@@ -202,3 +202,14 @@ def test_refused_arguments():
                    dict(pools=paged(data=pool.data.view(-1)[:8444 * 4].view(4, 8444))), dict(status_word=lengths.long())):
         with pytest.raises(wuda.WudaError):
             made(**change)
+
+
+def test_numbers_are_not_cut():
+    w = world(np.random.default_rng(7), 2, 4, LAYER, [32], [300] * 2, [64] * 2)
+    lengths, pool = plan_of(w).lengths, plan_of(w).pools[0]
+    paged = lambda **c: [wuda.PagedState(**dict(dict(data=pool.data, table=pool.table, entries_per_block=64, segments=(128, 4), tokens_per_entry=4), **c))]
+    wuda.BeamReorder(lengths, 4, pools=paged())
+    for width, pools in (((1 << 32) + 4, paged()), (4, paged(entries_per_block=(1 << 32) + 64)), (4, paged(segments=((1 << 32) + 128, 4))),
+                         (4, paged(tokens_per_entry=(1 << 32) + 4)), (4, paged(ring=1 << 32))):
+        with pytest.raises(wuda.WudaError):
+            wuda.BeamReorder(lengths, width, pools=pools)

@@ -210,3 +210,10 @@ def test_refused_arguments():
             bad()
     empty = wuda.beam_select(logits[:0], scores[:0], 4)
     assert [tuple(t.shape) for t in empty] == [(0, 4)] * 4
+
+
+def test_numbers_are_not_cut():
+    logits, scores = likely(2, 3, 50, "fp32", seed=0)
+    for bad in (dict(k=(1 << 32) + 4), dict(k=-(1 << 32) + 4), dict(eos_token=(1 << 32) + 4)):
+        with pytest.raises(wuda.WudaError):
+            wuda.beam_select(logits, scores, **bad)

@@ -315,3 +315,25 @@ def test_refused_arguments():
                    dict(lengths_out=d["lengths"][:2]), dict(status_word=d["lengths"].long()), dict(idx_entries_per_block=0)):
         with pytest.raises((wuda.WudaError, ZeroDivisionError)):
             made(**change)
+
+
+def test_what_a_step_writes_overlaps_nothing_and_numbers_are_not_cut():
+    s = state(np.random.default_rng(3), 4, 3, [1, 2, 3, 4], GEOMETRY, free=2)
+    d = {k: torch.from_numpy(v.copy()).cuda() for k, v in s.items()}
+    names = ("lengths", "idx_table", "cmp_table", "swa_table", "idx_free", "cmp_free", "free_counts")
+
+    def made(change={}, **more):
+        return wuda.StepTables(*[change.get(n, d[n]) for n in names], max_rows=2, **more)
+
+    block = torch.zeros(64, dtype=torch.int32, device="cuda")
+    made(dict(idx_free=block[:8], cmp_free=block[4:12]))                                  # only read: may overlap
+    made(lengths_out=d["lengths"], free_counts_out=block[:2])
+    made(lengths_out=block[4:8], free_counts_out=block[8:10], out=dict(n_compressed=block[:2], swa_lengths=block[2:4]))
+    for change, more in ((dict(lengths=block[:4]), dict(lengths_out=block[2:6])), (dict(), dict(free_counts_out=d["lengths"][:2])),
+                         (dict(), dict(out=dict(idx_block_table=d["idx_table"]))), (dict(), dict(out=dict(cmp_block_table=d["idx_table"]))),
+                         (dict(), dict(out=dict(n_compressed=block[:2], cmp_lengths=block[1:3]))),
+                         (dict(idx_free=block[:8]), dict(out=dict(n_compressed=block[6:8]))), (dict(idx_free=block), dict(lengths_out=block[60:])),
+                         (dict(), dict(topk=1 << 32)), (dict(), dict(window=(1 << 32) + 128)), (dict(), dict(max_tokens=1 << 32)),
+                         (dict(), dict(ring_entries=(1 << 32) + 8))):
+        with pytest.raises(wuda.WudaError):
+            made(change, **more)

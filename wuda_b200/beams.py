@@ -14,7 +14,7 @@ import torch
 from . import _lib
 from . import ops as _ops
 from ._lib import check, lib
-from .ops import _on_current_device, _require, _stream
+from .ops import _int32, _on_current_device, _require, _stream
 
 
 @dataclass
@@ -47,7 +47,7 @@ class BeamReorder:
         _require(status_word is None or (status_word.device == dev and status_word.dtype == torch.int32 and status_word.numel() >= 1),
                  "status_word must be int32 on the lengths' device")
         a = _lib.BeamReorderArgs(lengths=lengths.data_ptr(), num_states=len(states), num_pools=len(pools), capacity=capacity,
-                                 width=int(width), shared_lengths=None if shared_lengths is None else shared_lengths.data_ptr())
+                                 width=_int32(width, "width"), shared_lengths=None if shared_lengths is None else shared_lengths.data_ptr())
         for i, t in enumerate(states):
             _require(t.device == dev and t.is_contiguous() and t.dim() >= 1 and t.size(0) == capacity and t.numel() > 0,
                      "state %d must be contiguous [capacity, ...] on the lengths' device" % i)
@@ -60,9 +60,10 @@ class BeamReorder:
             _require(1 <= len(q.segments) <= 2, "a page has one or two segments")
             b = a.pools[i]
             b.data, b.table, b.stride_bytes = q.data.data_ptr(), q.table.data_ptr(), q.data.size(1)
-            b.num_blocks, b.table_width, b.entries_per_block = q.data.size(0), q.table.size(1), int(q.entries_per_block)
-            b.segment_bytes[0], b.segment_bytes[1] = int(q.segments[0]), int(q.segments[1]) if len(q.segments) > 1 else 0
-            b.tokens_per_entry, b.ring = int(q.tokens_per_entry), int(q.ring)
+            b.num_blocks, b.table_width, b.entries_per_block = q.data.size(0), q.table.size(1), _int32(q.entries_per_block, "entries_per_block")
+            for k, size in enumerate(q.segments):
+                b.segment_bytes[k] = _int32(size, "a segment")
+            b.tokens_per_entry, b.ring = _int32(q.tokens_per_entry, "tokens_per_entry"), _int32(q.ring, "ring")
         self.lengths, self.shared_lengths, self.states, self.pools = lengths, shared_lengths, list(states), list(pools)
         self.width, self.status_word = int(width), status_word
         self._device, self._args = dev.index, a

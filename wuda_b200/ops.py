@@ -216,6 +216,13 @@ _LOGITS_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _beam_scratch = Scratch(zeroed=True)     # the groups' counters, then the CTAs' lists and sums
 
 
+def _int32(value, name):
+    """value as the 32-bit integer that a C struct holds (ctypes would cut it off)."""
+    value = int(value)
+    _require(-(1 << 31) <= value < 1 << 31, "%s does not fit 32 bits" % name)
+    return value
+
+
 def _on_current_device(t):
     return t.is_cuda and t.device.index == torch._C._cuda_getDevice()
 
@@ -248,7 +255,8 @@ def beam_select(logits, scores, k=None, *, finished=None, eos_token=None):
                  tuple(finished.shape) == (groups, width), "finished must be contiguous bool [groups, width] on the logits' device")
         _require(eos_token is not None, "finished beams need an eos_token")
     _require(eos_token is None or 0 <= eos_token < vocab, "eos_token must be a token of the vocabulary")
-    k = width if k is None else int(k)
+    k = width if k is None else _int32(k, "k")
+    _int32(vocab, "the vocabulary")
     need = lib.wuda_beam_select_workspace_bytes(groups, width, vocab, k, _LOGITS_TYPES[logits.dtype])
     _require(need >= 0, "beam_select: groups <= 256, width in [1, 32], vocab in [1, 2^24] and k in [1, 64] are implemented")
     out = (scores.new_empty((groups, k)), scores.new_empty((groups, k), dtype=torch.int32),

@@ -15,7 +15,7 @@ from . import _lib
 from ._lib import check, lib
 from . import ops as _ops
 from .kv_cache import M1_BODY, RATIO, WIN
-from .ops import _on_current_device, _require, _stream
+from .ops import _int32, _on_current_device, _require, _stream
 
 _TOKEN_OUTPUTS = (("pos", torch.int64), ("q_pos", torch.int32), ("state_row", torch.int64), ("idx_dst", torch.int64),
                   ("cmp_dst", torch.int64), ("swa_dst", torch.int64))
@@ -36,6 +36,10 @@ class StepTables:
                  idx_entries_per_block=64, cmp_entries_per_block=64, swa_entries_per_block=256, ratio=4, ring_entries=8,
                  window=128, topk=2048, lengths_out=None, free_counts_out=None, out=None, status_word=None):
         max_tokens = max_rows if max_tokens is None else max_tokens
+        for value, name in ((max_rows, "max_rows"), (max_tokens, "max_tokens"), (idx_entries_per_block, "idx_entries_per_block"),
+                            (cmp_entries_per_block, "cmp_entries_per_block"), (swa_entries_per_block, "swa_entries_per_block"),
+                            (ratio, "ratio"), (ring_entries, "ring_entries"), (window, "window"), (topk, "topk")):
+            _int32(value, name)
         _require(max_rows >= 1 and max_tokens >= 0, "max_rows must be positive, max_tokens not negative")
         _require(_on_current_device(lengths), "the state must be on the current CUDA device")
         dev = lengths.device
@@ -85,6 +89,16 @@ class StepTables:
             self.out[name] = t
         _require(status_word is None or (status_word.device == dev and status_word.dtype == torch.int32 and status_word.numel() >= 1),
                  "status_word must be int32 on the lengths' device")
+        # what a step writes overlaps nothing else (rows are written while others are read), but the state may be its own successor
+        written = [idx_table, cmp_table, self.lengths_out, self.free_counts_out, *self.out.values()]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * 4 * (1 + (t.dtype is torch.int64)), i < len(written))
+                       for i, t in enumerate(written + [swa_table, idx_free, cmp_free] +
+                                             [t for t, after in ((lengths, self.lengths_out), (free_counts, self.free_counts_out))
+                                              if t.data_ptr() != after.data_ptr()]) if t.numel())
+        end, end_written = 0, 0
+        for begin, stop, writes in spans:
+            _require(begin >= (end if writes else end_written), "what a step writes must not overlap its other tensors")
+            end, end_written = max(end, stop), max(end_written, stop) if writes else end_written
         self.status_word = status_word
         self._device = dev.index
         p = lambda t: t.data_ptr()
