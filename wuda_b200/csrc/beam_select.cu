@@ -12,12 +12,24 @@
 // largest logit counts exactly 1, a row of one token has log-probability 0, and logits of any magnitude will do.  Which element a
 // thread gets depends on the element's number alone, not on the row's alignment, so equal rows have equal sums.
 //
-// Candidates: the k-th largest of 64 or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's k-th largest
-// logit, raised in front of the tiles 0, 3, 15, ..; what a thread has of a tile in which it sees a logit beyond the bound is noted (a
-// handful per tile) and looked at in the end, with the last bound.  No barrier besides.  A list that overflowed (sorted rows, rows of one value) is made again by exact selections.
+// Candidates: the k-th largest of 64 (k <= 32) or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's
+// k-th largest logit, raised in front of the tiles 0, 3, 15, .. (k > 32: 0, 1, 3, 7, ..); what a thread has of a tile in which it
+// sees a logit beyond the bound is noted (a handful per tile) and looked at in the end, with the last bound.  No barrier besides.  A
+// list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
-// The CTA that completes a group's counter merges its lists the same way: the k-th largest of the maxima over 128 shares of the entries
-// bounds what can be among the k best, and the few that pass are ranked by counting.
+// Rows that do not lie on 16 bytes: the aligned 16 bytes in which a vector begins are loaded as they are, and put together with the next
+// lane's when the tile is worked on, so that the loads stay in flight (the shift at the loads themselves would wait for them).
+//
+// The CTA that completes a group's counter merges its lists the same way: the k-th largest of the maxima over 64 or 128 shares of the
+// lists' first candidates bounds what can be among the k best, and the few that pass are ranked by counting.
+//
+// What bounds it (per launch in a graph, against a copy's 6.54 TB/s): small calls the chain of launch, a chunk's loads, its fence and
+// counter, and the merge's three round trips to L2 - 4 rows x 32000 bf16 8.3 us, of which the merge is 4.  Large ones the stream, and there
+// the issue slots beside it: 512 rows x 131072 bf16 (134 MB) 35.1 us, 20.5 at the copy's rate; the exponentials' unit is in use for 55 %
+// of the time, 0.59 instructions per cycle and scheduler, some 6 us of start and merge at both ends.  256 rows x 131072 fp32 take
+// 33 us, half the elements for the same bytes.  Rows off 16 bytes 41 us instead of 35.
+// More warps were worth more than anything else: a ring of bulk copies in shared memory left room for 5 or 6 CTAs per SM instead of 7
+// (49-54 us instead of 40 at the time), and exponentials by polynomials for a part of the elements took more slots than they freed (42-47).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
