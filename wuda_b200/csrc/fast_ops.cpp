@@ -2,7 +2,7 @@
 // current stream and the launch in one native call.  A call of an operator spends its host time on twenty attribute
 // reads, two or three allocations and a foreign-function call with a dozen arguments; the launch itself is 3 us of it.
 // Host time per call, one token, before -> after: rmsnorm_quant 12.4 -> 5.3 us, rope_quant 11.1 -> 4.4, act_quant 18.6 -> 6.4,
-// fp8_gemm 11.2 -> 6.4, topk 6.7 -> 2.2; norm + RoPE quantisation of 256 tokens, plain calls, 24.4 -> 13.1 us.
+// fp8_gemm 11.2 -> 6.4, topk 6.7 -> 2.2, beam_select 18.2 -> 7.5, step_tables 4.9 -> 3.3, beam_reorder 5.8 -> 3.2; norm + RoPE quantisation of 256 tokens, plain calls, 24.4 -> 13.1 us.
 //
 // Every function takes the arguments of the Python function of its name (ops.py), all positional, and either performs the
 // call or returns None, having done nothing: for arguments it does not know (another type of tensor, modes that
