@@ -13,7 +13,7 @@
 // thread gets depends on the element's number alone, not on the row's alignment, so equal rows have equal sums.
 //
 // Candidates: the k-th largest of 64 (k <= 32) or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's
-// k-th largest logit, raised in front of the tiles 0, 3, 15, .. (k > 32: 0, 1, 3, 7, ..); what a thread has of a tile in which it
+// k-th largest logit, raised in front of the tiles 0, 2, 8, 26, .. (k > 32: 0, 1, 3, 7, ..); what a thread has of a tile in which it
 // sees a logit beyond the bound is noted (a handful per tile) and looked at in the end, with the last bound.  No barrier besides.  A
 // list that overflowed (sorted rows, rows of one value) is made again by exact selections.
 //
@@ -24,12 +24,13 @@
 // lists' first candidates bounds what can be among the k best, and the few that pass are ranked by counting.
 //
 // What bounds it (per launch in a graph, against a copy's 6.54 TB/s): small calls the chain of launch, a chunk's loads, its fence and
-// counter, and the merge's three round trips to L2 - 4 rows x 32000 bf16 8.3 us, of which the merge is 4.  Large ones the stream, and there
-// the issue slots beside it: 512 rows x 131072 bf16 (134 MB) 35.1 us, 20.5 at the copy's rate; the exponentials' unit is in use for 55 %
-// of the time, 0.59 instructions per cycle and scheduler, some 6 us of start and merge at both ends.  256 rows x 131072 fp32 take
-// 33 us, half the elements for the same bytes.  Rows off 16 bytes 41 us instead of 35.
+// counter, and the merge's three round trips to L2 - 4 rows x 32000 bf16 8.2 us, of which the merge is 4.  Large ones the stream and what
+// goes on beside it: 512 rows x 131072 bf16 (134 MB) 32.6-33.7 us, 20.5 at the copy's rate.  Loads in this pattern alone take 22 us, the
+// exponentials 2 on top, raising the bounds and notes 2 each, the merge 4.  256 rows x 131072 fp32, half the elements for the same
+// bytes: 31.2.  Rows off 16 bytes: 38.9.
 // More warps were worth more than anything else: a ring of bulk copies in shared memory left room for 5 or 6 CTAs per SM instead of 7
 // (49-54 us instead of 40 at the time), and exponentials by polynomials for a part of the elements took more slots than they freed (42-47).
+// Asking L2 for the tiles after the next one made it slower (35.4 to 38.5 us for two to eight tiles ahead, against 35.0 at the time).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -207,7 +208,8 @@ static constexpr int kWarps = kThreads / 32, kNotes = kNotesOfBlock / kWarps, kN
 struct Shared {
     int count;                              // candidates (those beyond kList are lost)
     bool lost;                              // more was to be noted than there are places for
-    uint32_t bound, highest;                // the k-th largest logit so far, or less, and the largest, as ordered words
+    alignas(16) uint32_t bound[kWarps];     // the least is the k-th largest logit so far, or less, as an ordered word
+    uint32_t highest;                       // ... and the largest
     int hits[3];
     float warp_ref[kWarps];
     double warp_sum[kWarps];
@@ -336,34 +338,39 @@ static __device__ __noinline__ void candidates_exactly(Shared& sh, const T* row,
     }
 }
 
-// The k-th largest of 64 (k <= 32) or 128 words goes to *kth, the largest to *first.  Each word is looked at by `by` neighbouring
-// threads, which count a share of the others.  All threads, between two barriers of the caller's.
+// The k-th largest of 64 (k <= 32) or 128 words: the least of those with fewer than k larger ones.  Each word is looked at by `by`
+// neighbouring threads, which count a share of the others; every warp's least goes to `kth`, the largest of all to *first.  All
+// threads, between two barriers of the caller's; then least_of(kth).
 static __device__ __forceinline__ void kth_part(const uint32_t* parts, int k, uint32_t* kth, uint32_t* first) {
     const int tid = threadIdx.x, count = k <= 32 ? 64 : 128, by = kThreads / count, n = count / 4 / by;
     const uint32_t part = parts[tid / by];
     const uint4* share = reinterpret_cast<const uint4*>(parts) + tid % by * n;
-    int larger = 0, not_smaller = 0;
+    int larger = 0;
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
         const uint4 other = share[i];
         larger += (other.x > part) + (other.y > part) + (other.z > part) + (other.w > part);
-        not_smaller += (other.x >= part) + (other.y >= part) + (other.z >= part) + (other.w >= part);
     }
-    int both = larger | not_smaller << 16;
 #pragma unroll
     for (int o = 1; o < kThreads / 64; o <<= 1)
-        if (o < by) both += __shfl_xor_sync(0xffffffffu, both, o);
-    if ((both & 0xffff) < k && k <= both >> 16) *kth = part;      // (equal ones write the same)
-    if ((both & 0xffff) == 0) *first = part;
+        if (o < by) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+    if (larger == 0) *first = part;      // (equal ones write the same)
+    const uint32_t least = __reduce_min_sync(0xffffffffu, larger < k ? part : 0xffffffffu);
+    if ((tid & 31) == 0) kth[tid >> 5] = least;
+}
+static __device__ __forceinline__ uint32_t least_of(const uint32_t* kth) {
+    if constexpr (kWarps > 4) return __reduce_min_sync(0xffffffffu, kth[threadIdx.x % kWarps]);
+    const uint4 least = *reinterpret_cast<const uint4*>(kth);
+    return min(min(least.x, least.y), min(least.z, least.w));
 }
 
 // The k-th largest of maxima over all that some threads each have seen: k logits so far are at or above it.
 static __device__ __forceinline__ float raise_bound(Shared& sh, float so_far, int k, float bound, bool* raised) {
     atomicMax(&sh.part_max[threadIdx.x % (k <= 32 ? 64 : 128)], ordered(so_far));      // (what was there is of earlier tiles)
     __syncthreads();
-    kth_part(sh.part_max, k, &sh.bound, &sh.highest);
+    kth_part(sh.part_max, k, sh.bound, &sh.highest);
     __syncthreads();
-    const float now = unordered(sh.bound);
+    const float now = unordered(least_of(sh.bound));
     *raised = now > bound;
     return now;
 }
@@ -393,7 +400,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
             return;
         }
         const int at = element_of(tile, 0, lane) - back;
-        if (at - lane * kVec >= 0 && at + (kVectors * 32 + !ALIGNED - lane) * kVec <= a.vocab) {      // (of the whole warp)
+        if (ALIGNED || (at - lane * kVec >= 0 && at + (kVectors * 32 + 1 - lane) * kVec <= a.vocab)) {      // (of the whole warp)
 #pragma unroll
             for (int u = 0; u < kVectors; ++u) next[u] = load16(row + at + u * 32 * kVec);
             if constexpr (!ALIGNED) {
@@ -432,7 +439,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
     float ref = -FLT_MAX, so_far = -INFINITY, bound = -INFINITY;
     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
     int noted = 0;        // of the warp's vectors
-    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 3, 15, 63, .. or 0, 1, 3, 7, ..
+    int refresh = 0;      // the next tile in front of which the bound is raised: 0, 2, 8, 26, .. or 0, 1, 3, 7, ..
     for (int tile = 0; tile < tiles; ++tile) {
         uint32_t w[4 * kVectors];
         if (ALIGNED || off == 0 || tile >= whole) {
@@ -492,7 +499,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
         so_far = fmaxf(so_far, top);
         bool with_equal = false;      // a logit equal to the bound is a candidate where the bound is this tile's
         if (tile == refresh) {
-            refresh = k <= 32 ? 4 * refresh + 3 : 2 * refresh + 1;
+            refresh = k <= 32 ? 3 * refresh + 2 : 2 * refresh + 1;
             bound = raise_bound(sh, so_far, k, bound, &with_equal);
         }
         const bool hit = with_equal ? top >= bound : top > bound;
@@ -510,7 +517,7 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
 
     // ---- candidates: the noted elements that pass the last bound
     bool raised;
-    if ((k <= 32 ? 4 * (tiles - 1) + 3 : 2 * (tiles - 1) + 1) != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
+    if ((k <= 32 ? 3 * (tiles - 1) + 2 : 2 * (tiles - 1) + 1) != refresh) bound = raise_bound(sh, so_far, k, bound, &raised);
     else __syncthreads();      // (it was raised with the last tile)
     if (noted > kNotesAll) sh.lost = true;
     __syncwarp();
@@ -660,9 +667,9 @@ static __device__ __noinline__ void merge(Shared& sh, const Params& p, int g) {
     }
     if (part) atomicMax(&sh.front[tid % (k <= 32 ? 64 : 128)], part);
     __syncthreads();
-    kth_part(sh.front, k, &sh.bound, &sh.highest);
+    kth_part(sh.front, k, sh.bound, &sh.highest);
     __syncthreads();
-    const uint32_t least = max(sh.bound, 1u);
+    const uint32_t least = max(least_of(sh.bound), 1u);
     // the bound as a logit of each beam, a little lower (what is compared with it is rounded in other places)
     if (tid < a.width) {
         const double logit = unordered(least) - sh.score[tid] + sh.lse[tid];
@@ -789,11 +796,11 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
 
 // How the rows are cut, into chunks of whole tiles and lists that the merge can hold.
 //   Up to 148 rows of more work than a tile of 128 threads per SM: CTAs of 512 threads, one per SM at most.  Fewer and longer lists make
-//   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 12.3 us (14.2 in CTAs of 128), 128 rows x
-//   131072 bf16, k = 16: 17.6 (19.8); 64 rows x 131072 fp32, k = 4: 15.8 (16.0).
-//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 36.7 us in two chunks a row,
-//   39.0 in three, 49.3 with 512 threads; 4 rows x 32000 bf16: 8.7 us in eight chunks of a tile (9.6 with 512 threads).  Rows that
-//   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 55.3 -> 44.0 us.
+//   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 11.7 us (13.0 in CTAs of 128), 128 rows x
+//   131072 bf16, k = 16: 15.6 (17.4); 64 rows x 131072 fp32, k = 4: 13.0 (14.0).
+//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 32.6 us in two chunks a row,
+//   35.0 in three, 48.2 with 512 threads; 4 rows x 32000 bf16: 8.2 us in eight chunks of a tile (9.0 with 512 threads).  Rows that
+//   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 50.9 -> 39.7 us.
 struct Cut {
     int threads, chunks, chunk_vectors;
 };
