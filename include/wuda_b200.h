@@ -1056,7 +1056,8 @@ int wuda_indexer_topk_host_pages(wuda_indexer_plan* plan, const void* q_host, co
  * negative length or token count, pages beyond table_width, tokens beyond max_tokens (WUDA_DEV_BAD_LENGTH), and a row that needs
  * pages where the rows up to it need more than a stack holds (WUDA_DEV_NO_FREE_PAGE); rows behind it that need none are served.
  *
- * rows <= 4096, capacity <= 16384, max_tokens <= 262144, table_width <= 262144.
+ * rows <= 4096, capacity <= 16384, max_tokens <= 262144, table_width <= 262144.  A step of no rows writes the state where that is not
+ * in place (then token_starts[0], too), else nothing.
  */
 typedef struct wuda_step_tables_args {
     const int32_t* lengths;      /* int32 [capacity]: tokens that each slot's caches hold                */

@@ -337,3 +337,19 @@ def test_what_a_step_writes_overlaps_nothing_and_numbers_are_not_cut():
                          (dict(), dict(ring_entries=(1 << 32) + 8))):
         with pytest.raises(wuda.WudaError):
             made(change, **more)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_step_of_no_rows_carries_the_state_over(in_place):
+    s = state(np.random.default_rng(5), 9, 3, [1, 2, 3, 4, 5, 6, 7, 8, 300], GEOMETRY, free=2)
+    plan = plan_of(s, 4, 4, GEOMETRY, in_place)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    want = oracle(s, np.zeros(0, np.int32), None, 4, GEOMETRY)
+    for new in (None, none):
+        plan.lengths_out.fill_(-7) if not in_place else None
+        plan.step(none, new)
+        torch.cuda.synchronize()
+        assert np.array_equal(plan.lengths_out.cpu().numpy(), want["lengths"]) and np.array_equal(plan.free_counts_out.cpu().numpy(), want["counts"])
+        assert plan.out["token_starts"][1:].eq(-99).all() and (in_place or int(plan.out["token_starts"][0]) == 0)
+        assert all(plan.out[name].eq(-99).all() for name in TOKEN + ROW)
+    assert int(plan._counter) == 0

@@ -290,8 +290,8 @@ extern "C" int wuda_step_tables(const wuda_step_tables_args* args, const int32_t
                  "token outputs must not be NULL");
     WUDA_REQUIRE((a.idx_free || a.idx_free_capacity == 0) && (a.cmp_free || a.cmp_free_capacity == 0), "free stacks must not be NULL");
     WUDA_REQUIRE(a.idx_table != a.cmp_table, "the two pools must not share a page table");
-    if (rows == 0) return WUDA_OK;
-    WUDA_REQUIRE(slots, "slots must not be NULL");
+    if (rows == 0 && a.lengths_out == a.lengths && a.free_counts_out == a.free_counts) return WUDA_OK;      // (there is nothing to write)
+    WUDA_REQUIRE(slots || rows == 0, "slots must not be NULL");
     DeviceInfo dev;
     if (const int st = current_device_info(&dev)) return st;
     const size_t smem = shared_bytes(rows, a.capacity);
@@ -302,9 +302,9 @@ extern "C" int wuda_step_tables(const wuda_step_tables_args* args, const int32_t
     p.ratio = Divisor(a.ratio), p.ring = Divisor(a.ring_entries), p.window = Divisor(a.window);
     p.idx_epb = Divisor(a.idx_entries_per_block), p.cmp_epb = Divisor(a.cmp_entries_per_block), p.swa_epb = Divisor(a.swa_entries_per_block);
     p.pieces = Divisor((a.table_width + kPiece - 1) / kPiece);
-    const int64_t tokens = new_tokens ? a.max_tokens : rows;
+    const int64_t tokens = new_tokens && rows ? a.max_tokens : rows;
     const int64_t tasks = static_cast<int64_t>(rows) * (2 * ((a.table_width + kPiece - 1) / kPiece) + 1) + (tokens + 31) / 32;
-    const int grid = static_cast<int>(tasks < static_cast<int64_t>(dev.num_sms) * kWarps ? (tasks + kWarps - 1) / kWarps : dev.num_sms);
+    const int grid = static_cast<int>(tasks < static_cast<int64_t>(dev.num_sms) * kWarps ? (tasks + kWarps - 1) / kWarps + (tasks == 0) : dev.num_sms);
     WUDA_CUDA(launch_pdl(step_tables_kernel, dim3(grid), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p));
     return WUDA_OK;
 }
