@@ -217,3 +217,18 @@ def test_numbers_are_not_cut():
     for bad in (dict(k=(1 << 32) + 4), dict(k=-(1 << 32) + 4), dict(eos_token=(1 << 32) + 4)):
         with pytest.raises(wuda.WudaError):
             wuda.beam_select(logits, scores, **bad)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab", [50, 9001, 70001])
+def test_zeros_of_both_signs_are_equal(kind, vocab):
+    """The best logits are zeros, signs by turns: the lower token first; scores of both signs: the lower beam."""
+    logits = torch.full((2, 3, vocab), -4.0, dtype=TYPES[kind], device="cuda")
+    logits[:, :, 5::3] = -0.0
+    logits[:, :, 7::6] = 0.0
+    logits[1, :, 40:] = logits[1, :, 40:].flip(-1)
+    scores = torch.tensor([[-0.0, 0.0, -0.0], [-0.0, 0.0, 0.0]], device="cuda")
+    for k in (1, 11, 40):
+        check(wuda.beam_select(logits, scores, k), logits, scores, k, exact=True)
+    ended = torch.ones(2, 3, dtype=torch.bool, device="cuda")
+    check(wuda.beam_select(logits, scores, 3, finished=ended, eos_token=4), logits, scores, 3, ended, 4, exact=True)

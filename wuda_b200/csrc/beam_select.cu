@@ -97,7 +97,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
-__device__ __forceinline__ Key key_of(float x, uint32_t token) { return (static_cast<Key>(ordered(x)) << 32) | ~token; }
+__device__ __forceinline__ Key key_of(float x, uint32_t token) { return (static_cast<Key>(ordered(x + 0.f)) << 32) | ~token; }      // (-0 counts as 0)
 __device__ __forceinline__ uint32_t token_of(Key k) { return ~static_cast<uint32_t>(k); }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -195,7 +195,7 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) {       // of a 16-bit typ
 }
 // a word that grows with the value; 0 is below every number
 __device__ __forceinline__ Key ordered(double x) {
-    const long long b = __double_as_longlong(x);
+    const long long b = __double_as_longlong(x + 0.);      // (-0 counts as 0)
     return static_cast<Key>(b) ^ (static_cast<Key>(b >> 63) | (1ull << 63));
 }
 __device__ __forceinline__ double unordered(Key u) { return __longlong_as_double(u & (1ull << 63) ? u ^ (1ull << 63) : ~u); }
