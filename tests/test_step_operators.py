@@ -177,3 +177,28 @@ def test_a_fork_without_room_takes_nothing():
     assert m.fork_request(a, 0) == [] and not m.reqs[a].get("shared")
     (b,) = m.fork_request(a, 1)
     assert m.reqs[b]["cmp"][0] == m.reqs[a]["cmp"][0]
+
+
+@pytest.mark.parametrize("tokens", [0, 100, 1000])
+def test_what_is_left_of_a_fork_is_forked_again(tokens):
+    """The winner of a search goes on alone and starts the next one; until then no member of the fork starts one of its own."""
+    m = KVCacheManager(5, 30, 30, device="cpu")
+    a = m.alloc_request()
+    m.advance(a, tokens)
+    b, c = m.fork_request(a, 2)
+    for freed in (a, c):
+        with pytest.raises(ValueError):
+            m.fork_request(b, 1)
+        m.free_request(freed)
+    for _ in range(300):
+        m.step_begin([b])
+    d, e = m.fork_request(b, 2)
+    filled = (tokens + 300) // 4 // 64
+    for s in (d, e):
+        assert m.reqs[s]["shared"] == m.reqs[b]["shared"] == tokens + 300 and m.reqs[s]["cmp"][:filled] == m.reqs[b]["cmp"][:filled]
+        assert not set(m.reqs[s]["cmp"][filled:]) & set(m.reqs[b]["cmp"])
+    for s in (d, b, e):
+        m.free_request(s)
+    assert not m._owners["cmp"] and not m._owners["idx"]
+    for name in ("swa", "cmp", "idx"):
+        assert sorted(m._pools[name]._free) == list(range(30))

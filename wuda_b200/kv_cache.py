@@ -84,7 +84,8 @@ class KVCacheManager:
         for slot in range(capacity):
             self._reset_state(slot)
         self._free_slots = list(range(capacity - 1, -1, -1))
-        self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables, "shared": tokens in shared pages}
+        self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables, "shared": tokens in shared pages,
+                                # "group": the slots that share them}
         self._owners = {"cmp": {}, "idx": {}}      # page -> requests that hold it, where they are more than one
         self.on_device = False  # step tables on the device (step_tables.CacheTables) have the requests' state: nothing changes here
 
@@ -125,6 +126,11 @@ class KVCacheManager:
         for name in ("swa", "cmp", "idx"):
             self._pools[name].give_back(self._given_up(name, req[name]))
         self._free_slots.append(slot)
+        group = req.get("group", set())
+        group.discard(slot)
+        if len(group) == 1:     # what the last of them holds is its own
+            last = self.reqs[group.pop()]
+            del last["shared"], last["group"]
 
     def _given_up(self, name, pages):
         """Those of a request's pages that no other request holds any longer."""
@@ -145,11 +151,12 @@ class KVCacheManager:
     def fork_request(self, slot, copies):
         """`copies` new requests that continue request `slot` (the beams of a prompt; not in the reference's manager).  Returns
         their slots.  All of them, the request included, share its filled compressed pages; state rings, window pages and
-        the compressed page that is being filled are copied.  A request that shares pages already is not forked again."""
+        the compressed page that is being filled are copied.  A request is not forked again before the others of its fork are
+        free."""
         self._need_state()
         req = self.reqs[slot]
-        if req.get("shared"):
-            raise ValueError("request %d shares its pages already" % slot)
+        if "group" in req:
+            raise ValueError("request %d is one of a fork already" % slot)
         entries = (req["pos"] + 1) // RATIO
         own = {name: len(req[name]) - min(entries // self.entries_per_block[name], len(req[name])) for name in ("cmp", "idx")}
         if copies < 0 or copies > len(self._free_slots) or any(
@@ -172,6 +179,9 @@ class KVCacheManager:
             slots.append(new)
         if copies:
             req["shared"] = req["pos"] + 1
+            group = {slot, *slots}
+            for member in group:
+                self.reqs[member]["group"] = group
         return slots
 
     # ---- one decode step: positions, state rows and cache destinations of every request
