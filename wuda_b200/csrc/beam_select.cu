@@ -8,8 +8,8 @@
 //
 // One launch.  A row of logits is cut into chunks, a CTA each, that are read once: 16 bytes per load, four loads per thread ahead of the
 // four that it works on.  Every thread keeps a reference r and the sum of exp(x - r) of its elements; r follows the maximum only where a
-// term would pass e^40, so a rescaling is rare and no term overflows.  x - r is formed before the product with log2 e: the
-// largest logit counts exactly 1, a row of one token has log-probability 0, and logits of any magnitude will do.  Which element a
+// term would pass e^40, so a rescaling is rare and no term overflows.  x - r is formed before the product with log2 e: a
+// logit equal to r counts exactly 1, a row of one token has log-probability 0, and logits of any magnitude will do.  Which element a
 // thread gets depends on the element's number alone, not on the row's alignment, so equal rows have equal sums.
 //
 // Candidates: the k-th largest of 64 (k <= 32) or 128 maxima over disjoint parts of the tiles so far is a lower bound of the chunk's
