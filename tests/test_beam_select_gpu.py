@@ -232,3 +232,11 @@ def test_zeros_of_both_signs_are_equal(kind, vocab):
         check(wuda.beam_select(logits, scores, k), logits, scores, k, exact=True)
     ended = torch.ones(2, 3, dtype=torch.bool, device="cuda")
     check(wuda.beam_select(logits, scores, 3, finished=ended, eos_token=4), logits, scores, 3, ended, 4, exact=True)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("groups, width, vocab, k", [(5, 32, 9001, 64), (9, 31, 20011, 62), (6, 32, 33000, 32), (13, 31, 8300, 33), (14, 30, 8300, 34)])
+def test_wide_groups_with_long_lists(groups, width, vocab, k, kind):
+    """One or two chunks to a row because the merge holds no more lists, on both sides of the rule for the size of the CTAs."""
+    logits, scores = likely(groups, width, vocab, kind, seed=groups * k)
+    check(wuda.beam_select(logits, scores, k), logits, scores, k)

@@ -798,6 +798,8 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
 //   Up to 148 rows of more work than a tile of 128 threads per SM: CTAs of 512 threads, one per SM at most.  Fewer and longer lists make
 //   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 11.7 us (13.0 in CTAs of 128), 128 rows x
 //   131072 bf16, k = 16: 15.6 (17.4); 64 rows x 131072 fp32, k = 4: 13.0 (14.0).
+//   So, too, where the lists leave fewer than two fifths of the places of CTAs of 128 threads (wide groups, large k): 8 x 32 rows x
+//   131072 bf16, k = 64: 41.7 us (47.9 in CTAs of 128), 6 x 32 rows, k = 32: 28.2 (35.0); at half of them, 16 x 32 rows, k = 64, 76.3 (58.4).
 //   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 32.6 us in two chunks a row,
 //   35.0 in three, 48.2 with 512 threads; 4 rows x 32000 bf16: 8.2 us in eight chunks of a tile (9.0 with 512 threads).  Rows that
 //   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 50.9 -> 39.7 us.
@@ -807,12 +809,16 @@ struct Cut {
 Cut cut(int groups, int width, int vocab, int k, int type) {
     const int rows = groups * width, of_128 = (type == 2 ? 4 : 8) * kVectors * 128;
     Cut c = {};
-    c.threads = rows <= kSms && static_cast<int64_t>(rows) * ((vocab + of_128 - 1) / of_128) > kSms ? 512 : 128;
+    const int tiles_of_128 = (vocab + of_128 - 1) / of_128;
+    const int held = std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k));      // chunks of a row that the merge can hold
+    const bool few_rows = rows <= kSms && static_cast<int64_t>(rows) * tiles_of_128 > kSms;
+    const bool few_lists = held < tiles_of_128 && rows * held * 5 < 7 * kSms * 2;
+    c.threads = few_rows || few_lists ? 512 : 128;
     const int tile = of_128 * (c.threads / 128), tiles = (vocab + tile - 1) / tile;
     const int resident = (c.threads == 512 ? 1 : 7) * kSms;
     int n = std::max(resident / rows, 1);
     if (n == 1 && rows * 5 < resident * 4 && tiles >= 6) n = 3;
-    n = std::min(std::min(n, tiles), std::min(std::min(kMostChunks, kMostLists / width), kEntries / (width * k)));
+    n = std::min(std::min(n, tiles), held);
     const int per = (tiles + n - 1) / n;
     c.chunks = (tiles + per - 1) / per;
     c.chunk_vectors = per * c.threads * kVectors;
