@@ -240,3 +240,56 @@ def test_wide_groups_with_long_lists(groups, width, vocab, k, kind):
     """One or two chunks to a row because the merge holds no more lists, on both sides of the rule for the size of the CTAs."""
     logits, scores = likely(groups, width, vocab, kind, seed=groups * k)
     check(wuda.beam_select(logits, scores, k), logits, scores, k)
+
+
+COUNTS = (383, 385, 1023, 1024, 1025, 1200, 1366, 1536, 1537, 2050)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("groups, vocab", [(10, 131072), (10, 8192), (2, 131072)])
+def test_as_many_candidates_as_a_list_holds_and_more(groups, vocab, pad, kind):
+    """One group each with so many equal maxima in one chunk, and with so many tokens in front that are not masked: what is ranked as
+    it is, trimmed, and selected exactly, in CTAs of 512 threads (10 rows of 131072) and of 128."""
+    for first in range(0, len(COUNTS), groups):
+        counts = COUNTS[first:first + groups]
+        held = torch.full((groups, 1, vocab + pad), -3.0, dtype=TYPES[kind], device="cuda")
+        logits = held[:, :, :vocab]
+        scores = torch.full((groups, 1), -2.5, device="cuda")
+        for g, n in enumerate(counts):       # spread over as many threads of a tile as there are
+            logits[g, 0, :min(vocab, 8192) // n * n:min(vocab, 8192) // n] = 2.0
+        for k in (4, 64):
+            got = wuda.beam_select(logits, scores, k)
+            check(got, logits, scores, k, exact=True)
+            for a, b in zip(got, wuda.beam_select(logits, scores, k)):
+                assert torch.equal(a, b)
+        logits.copy_(torch.round(likely(groups, 1, vocab, kind, seed=first)[0] * 4) / 4)
+        for g, n in enumerate(counts):
+            logits[g, 0, n:] = float("-inf")
+        for k in (4, 64):
+            check(wuda.beam_select(logits, scores, k), logits, scores, k, exact=True)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_full_lists_of_several_beams(kind):
+    """Every sixth of the first tokens at one maximum, in all beams of all groups; few tokens of many allowed, in wide groups."""
+    logits = torch.full((16, 4, 131072), -3.0, dtype=TYPES[kind], device="cuda")
+    logits[:, :, 0:8191:6] = 2.0
+    scores = torch.full((16, 4), -1.25, device="cuda")
+    check(wuda.beam_select(logits, scores, 4), logits, scores, 4, exact=True)
+    for allowed in (1100, 1500):
+        logits, scores = likely(1, 32, 131072, kind, seed=allowed)
+        logits[:, :, allowed:] = float("-inf")
+        check(wuda.beam_select(logits, scores, 64), logits, scores, 64)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_of_one_value_and_sorted_rows_in_large_blocks(kind):
+    vocab = 131072
+    up = torch.linspace(-30, 30, vocab)
+    rows = torch.stack([torch.zeros(vocab), torch.full((vocab,), torch.finfo(TYPES[kind]).min), torch.full((vocab,), torch.finfo(TYPES[kind]).max),
+                        up, up.flip(0), up.abs(), -up.abs()])
+    logits = rows.to(TYPES[kind]).cuda().view(7, 1, vocab)
+    scores = torch.full((7, 1), -0.75, device="cuda")
+    for k in (5, 40):
+        check(wuda.beam_select(logits, scores, k), logits, scores, k, exact=True)

@@ -204,6 +204,8 @@ __device__ __forceinline__ double unordered(Key u) { return __longlong_as_double
 template <int kThreads>
 struct Block {
 static constexpr int kWarps = kThreads / 32, kNotes = kNotesOfBlock / kWarps, kNotesAll = kNotesAllOfBlock / kWarps;
+// Candidates that are ranked side by side, a few per thread; beyond that the list is trimmed first.  It holds no more than kList.
+static constexpr int kRanked = 3 * kThreads < kList ? 3 * kThreads : kList;
 
 struct Shared {
     int count;                              // candidates (those beyond kList are lost)
@@ -559,10 +561,10 @@ static __device__ __forceinline__ void chunk(Shared& sh, const Params& p, const 
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) sh.warp_sum[warp] = total;
-    if (sh.count > 3 * kThreads || sh.lost) {
+    if (sh.count > kRanked || sh.lost) {
         const bool lost = sh.count > kList || sh.lost;
         __syncthreads();
-        if (lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
+        if (kRanked == kList || lost) candidates_exactly<T>(sh, row, c0, end, a.vocab, k);
         else trim_list(sh, k);      // more than ranking each takes
     } else {
         __syncthreads();
