@@ -353,3 +353,26 @@ def test_a_step_of_no_rows_carries_the_state_over(in_place):
         assert plan.out["token_starts"][1:].eq(-99).all() and (in_place or int(plan.out["token_starts"][0]) == 0)
         assert all(plan.out[name].eq(-99).all() for name in TOKEN + ROW)
     assert int(plan._counter) == 0
+
+
+def test_making_a_plan_launches_nothing():
+    """A plan whose next state is not in place: what the caller holds there is written by its steps alone, on their stream."""
+    s = state(np.random.default_rng(6), 9, 3, [1, 2, 3, 4, 5, 6, 7, 8, 300], GEOMETRY, free=4)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    plan_of(s, 4, 4, GEOMETRY, False)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        plan = plan_of(s, 4, 4, GEOMETRY, False)
+    torch.cuda.synchronize()
+    assert plan.lengths_out.eq(-7).all() and plan.free_counts_out.eq(-7).all()
+    slots = np.array([3, 8, 0], np.int32)
+    dev, want = torch.from_numpy(slots).cuda(), oracle(s, slots, None, 4, GEOMETRY)
+    d = {k: torch.from_numpy(v.copy()).cuda() for k, v in s.items()}
+    after = torch.full_like(d["lengths"], -7), torch.full_like(d["free_counts"], -7)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):            # made while a graph is captured, too
+        plan = wuda.StepTables(d["lengths"], d["idx_table"], d["cmp_table"], d["swa_table"], d["idx_free"], d["cmp_free"], d["free_counts"],
+                               max_rows=4, topk=GEOMETRY["topk"], lengths_out=after[0], free_counts_out=after[1])
+        plan.step(dev)
+    graph.replay()
+    check(plan, want, 3, untouched=False)

@@ -112,7 +112,10 @@ class StepTables:
             **{name: p(t) for name, t in self.out.items()})
         self._args_ref, self._address = ctypes.byref(self._args), ctypes.addressof(self._args)
         self._status = None if status_word is None else status_word.data_ptr()
-        check(lib.wuda_step_tables(self._args_ref, None, None, 0, None, None))
+        # the library's checks: a call of no rows launches nothing where the state is in place
+        checked = _lib.StepTablesArgs.from_buffer_copy(self._args)
+        checked.lengths_out, checked.free_counts_out = checked.lengths, checked.free_counts
+        check(lib.wuda_step_tables(ctypes.byref(checked), None, None, 0, None, None))
 
     def step(self, slots, new_tokens=None):
         """slots int32 [rows]: the request slot of each row, -1 for a padded row, each slot once; new_tokens int32 [rows]: its
