@@ -1,4 +1,8 @@
 """Beam reordering against the definition, entry by entry.  Bytes have to be equal, those that no fork touches included."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -213,3 +217,32 @@ def test_numbers_are_not_cut():
                          (4, paged(tokens_per_entry=(1 << 32) + 4)), (4, paged(ring=1 << 32))):
         with pytest.raises(wuda.WudaError):
             wuda.BeamReorder(lengths, width, pools=pools)
+
+
+WHERE_SHARED_MEMORY_PASSES_48_KB = """
+import torch
+import wuda_b200 as wuda
+
+# (8 x beams + capacity) x 4 bytes for the plan beside what a CTA has in any case: the first call of each size in a process that has
+# made no larger one
+for groups, width, capacity in ((1, 4, 11700), (1, 4, 11836), (1, 4, 11837), (128, 8, 3690), (128, 8, 3800), (1, 4, 11900), (100, 10, 4032),
+                                (1, 4, 12000), (1, 4, 12001), (128, 8, 3841), (128, 32, 16384)):
+    beams = groups * width
+    state = torch.arange(capacity * 3, dtype=torch.int32, device="cuda").view(capacity, 3)
+    want = state.clone()
+    lengths = torch.full((capacity,), 5, dtype=torch.int32, device="cuda")
+    slots = torch.randperm(capacity, device="cuda")[:beams].int().view(groups, width)
+    parents = torch.zeros(groups, width, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(slots)
+    wuda.BeamReorder(lengths, width, states=[state]).run(parents, slots, out)
+    want[slots.view(-1).long()] = want[slots[:, :1].expand(groups, width).reshape(-1).long()]
+    assert torch.equal(out, slots) and torch.equal(state, want), (groups, width, capacity)
+print("all sizes")
+"""
+
+
+def test_sizes_around_the_shared_memory_of_a_plain_launch():
+    """In a process of its own: a larger call before would have asked for more shared memory for good."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", WHERE_SHARED_MEMORY_PASSES_48_KB], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "all sizes" in run.stdout, run.stderr[-2000:]

@@ -38,6 +38,7 @@ struct Params {
 };
 
 inline size_t shared_bytes(int rows, int capacity) { return sizeof(int) * (8ull * rows + capacity); }
+constexpr size_t kPlainBytes = 44 * 1024;    // of 48 KB that a launch may take without asking: the rest holds the static arrays
 
 // The n-th lowest member of a set, -1 where there are fewer: halves, by their members.
 __device__ __forceinline__ int lowest_but(uint32_t set, int n) {
@@ -112,6 +113,7 @@ __global__ void __launch_bounds__(kThreads, kResident) beam_reorder_kernel(const
     extern __shared__ int mem[];
     __shared__ int scan[33];
     __shared__ Piece pieces[kBatch];
+    static_assert(sizeof scan + sizeof pieces + 16 <= 48 * 1024 - kPlainBytes, "static and dynamic shared memory pass 48 KB together");
     const wuda_beam_reorder_args& a = p.a;
     const int width = a.width, rows = p.groups * width, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int* slot = mem;                 // of the beams now
@@ -330,7 +332,7 @@ extern "C" int wuda_beam_reorder(const wuda_beam_reorder_args* args, const int32
     if (const int st = current_device_info(&dev)) return st;
     const int rows = beams;
     const size_t smem = shared_bytes(rows, a.capacity);
-    if (smem > 48 * 1024 - 1024)
+    if (smem > kPlainBytes)
         WUDA_CUDA(cudaFuncSetAttribute(beam_reorder_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(shared_bytes(kMostRows, kMostSlots))));
     const int64_t most = pieces * rows;
