@@ -376,3 +376,24 @@ def test_making_a_plan_launches_nothing():
         plan.step(dev)
     graph.replay()
     check(plan, want, 3, untouched=False)
+
+
+def test_beams_move_only_while_the_tables_have_the_state():
+    """Between a pull() and the next push() the pages in the tables may be other requests' already."""
+    cache = KVCacheManager(4, 12, 4)
+    a = cache.alloc_request()
+    cache.advance(a, 300)
+    tables = CacheTables(cache, 4)
+    reorder = tables.beam_reorder(2)
+    pair = lambda *v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    out = pair(-5, -5)
+    tables.pull()
+    (b,) = cache.fork_request(a, 1)
+    with pytest.raises(wuda.WudaError):
+        reorder.run(pair(0, 0), pair(a, b), out)
+    torch.cuda.synchronize()
+    assert out.tolist() == [[-5, -5]]
+    tables.push()
+    cache.main_state[a] = 3.0
+    reorder.run(pair(0, 0), pair(a, b), out)
+    assert out.tolist() == [[a, b]] and torch.all(cache.main_state[b] == 3.0)

@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from ._lib import check, lib
 from . import ops as _ops
+from .beams import BeamReorder, PagedState
 from .kv_cache import M1_BODY, RATIO, WIN
 from .ops import _int32, _on_current_device, _require, _stream
 
@@ -209,12 +210,25 @@ class CacheTables(StepTables):
         return super().step(slots, new_tokens)
 
     def beam_reorder(self, width, states=(), status_word=None):
-        """A BeamReorder over the cache's state rings and pools, and `states` beside them ([capacity, ...] by slot)."""
-        from .beams import BeamReorder, PagedState
+        """A BeamReorder over the cache's state rings and pools, and `states` beside them ([capacity, ...] by slot).  Like a step, it
+        runs from a push() to the next pull()."""
         cache = self.cache
         epb, key = cache.entries_per_block, cache.idx_entry_bytes - 4
         pools = [PagedState(cache.idx_pool, self.idx_table, epb["idx"], (key, 4), tokens_per_entry=RATIO),
                  PagedState(cache.cmp_pool, self.cmp_table, epb["cmp"], (M1_BODY, 8), tokens_per_entry=RATIO),
                  PagedState(cache.swa_pool, self.swa_table, epb["swa"], (M1_BODY, 8), ring=WIN)]
-        return BeamReorder(self.lengths, width, shared_lengths=self.shared_lengths, states=[cache.main_state, cache.idx_state, *states],
-                           pools=pools, status_word=self.status_word if status_word is None else status_word)
+        return _CacheReorder(self, width, states=[cache.main_state, cache.idx_state, *states], pools=pools,
+                             status_word=self.status_word if status_word is None else status_word)
+
+
+class _CacheReorder(BeamReorder):
+    """The beams of a KVCacheManager's requests.  While the manager has their state, the pages in the tables may be others'."""
+
+    def __init__(self, tables, width, **more):
+        super().__init__(tables.lengths, width, shared_lengths=tables.shared_lengths, **more)
+        self._tables = tables
+
+    def run(self, parents, slots, slots_out):
+        if not self._tables._pushed:
+            raise _lib.WudaError(1, "the cache manager has the state: push() it first")
+        return super().run(parents, slots, slots_out)
