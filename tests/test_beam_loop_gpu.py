@@ -220,3 +220,20 @@ def test_a_beam_search_moves_whole_requests(captured):
     assert pos == {cache.reqs[s]["pos"] for g in mine for s in g}
     assert got[1].view(groups, width, steps).tolist() == tokens
     assert torch.equal(got[0], scores) and torch.equal(got[2], logits) and torch.equal(got[3], finished)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_capture_that_fails_leaves_the_requests_where_they_were(native):
+    layer, slots, x = build_random_layer(3, 250, seed=37, native=native, **SMALL)
+    dev = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    tables = layer.device_tables()
+    before = tables.lengths.tolist(), tables.free_counts.tolist()
+    for bad in (x[:, :2], x.float(), x.transpose(0, 1)):
+        with pytest.raises((ValueError, RuntimeError)):
+            layer.capture(bad, 3, slots=dev)
+        assert (tables.lengths.tolist(), tables.free_counts.tolist()) == before
+    layer.capture(x, 3, slots=dev)
+    layer.replay()
+    torch.cuda.synchronize()
+    layer.check_status()
+    assert tables.lengths.tolist() == [n + 1 for n in before[0]]

@@ -306,17 +306,20 @@ class DecoderLayer:
         """One eager pass, then the same pass as a CUDA graph reading `hidden_states` in place.  On a pair of
         ranks both must call this (and later replay()) the same number of times: the exchange steps number
         their calls on the device.  With slots (int32 [m] on the device) the graph prepares its step itself
-        (prepare_on_device), so that every replay is the next token; the eager pass is taken back."""
+        (prepare_on_device), so that every replay is the next token; the eager pass is taken back, also where it fails."""
         if slots is not None:
             if slots.numel() != m:
                 raise ValueError("slots must be one for each of the %d rows" % m)
             tables = self.device_tables()
             before = tables.lengths.clone(), tables.free_counts.clone()
-            self.prepare_on_device(slots)
-        self.launch(hidden_states, m)
-        if slots is not None:      # (the pages it took are the ones that the first replay takes, and what it wrote is written again)
-            tables.lengths.copy_(before[0])
-            tables.free_counts.copy_(before[1])
+        try:
+            if slots is not None:
+                self.prepare_on_device(slots)
+            self.launch(hidden_states, m)
+        finally:
+            if slots is not None:      # (the pages it took are the ones that the first replay takes, and what it wrote is written again)
+                tables.lengths.copy_(before[0])
+                tables.free_counts.copy_(before[1])
         torch.cuda.synchronize()
         self.check_status()
         graph = torch.cuda.CUDAGraph()
