@@ -5,6 +5,7 @@ import torch
 
 import wuda_b200 as wuda
 from wuda_b200.layer_setup import build_random_layer
+from wuda_b200.step_tables import CacheTables
 
 pytestmark = pytest.mark.gpu
 SMALL = dict(topk=512, experts=32, inter=512, moe_topk=4)
@@ -237,3 +238,23 @@ def test_a_capture_that_fails_leaves_the_requests_where_they_were(native):
     torch.cuda.synchronize()
     layer.check_status()
     assert tables.lengths.tolist() == [n + 1 for n in before[0]]
+
+
+def test_a_graph_steps_only_from_the_state_of_its_own_tables():
+    """Two tables over one cache: while the other ones have its state, a graph of the layer's would step from an old one."""
+    layer, slots, x = build_random_layer(2, 250, seed=41, **SMALL)
+    dev = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    tables = layer.device_tables()
+    layer.capture(x, 2, slots=dev)
+    layer.replay()
+    tables.pull()
+    other = CacheTables(layer.attn.cache, 2)
+    other.step(dev)
+    with pytest.raises(RuntimeError):
+        layer.replay()
+    other.pull()
+    tables.push()
+    layer.replay()
+    torch.cuda.synchronize()
+    layer.check_status()
+    assert tables.lengths.tolist() == [252, 252]

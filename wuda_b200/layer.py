@@ -331,8 +331,8 @@ class DecoderLayer:
         return graph
 
     def replay(self):
-        if self._graph_slots is not None and not self.attn.cache.on_device:
-            raise RuntimeError("the graph prepares its steps from the device's state: push() it first")
+        if self._graph_slots is not None and not self.device_tables().has_state:
+            raise RuntimeError("the graph prepares its steps from the state in the layer's tables on the device: push() it first")
         self._graph.replay()
         return self._graph_out
 

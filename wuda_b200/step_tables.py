@@ -156,7 +156,7 @@ class CacheTables(StepTables):
         epb = cache.entries_per_block
         pages = {name: cache._pools[name].data.size(0) for name in ("idx", "cmp")}
         self.shared_lengths = i32(cache.capacity)
-        self._pushed = False        # who has the state: these tables, from a push() to the next pull(), or the manager
+        self.has_state = False      # these tables have the state, from a push() to the next pull(); else the manager has it, or other tables
         super().__init__(i32(cache.capacity), i32(cache.capacity, cache.max_pages), i32(cache.capacity, cache.max_pages),
                          i32(cache.capacity, -(-WIN // epb["swa"])), i32(pages["idx"]), i32(pages["cmp"]), i32(2),
                          max_rows=max_rows, max_tokens=max_tokens, idx_entries_per_block=epb["idx"],
@@ -186,12 +186,12 @@ class CacheTables(StepTables):
         self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
         self.shared_lengths.copy_(torch.tensor(shared, dtype=torch.int32))
         self.free_counts.copy_(torch.tensor([len(cache._pools[name]._free) for name in ("idx", "cmp")], dtype=torch.int32))
-        cache.on_device = self._pushed = True
+        cache.on_device = self.has_state = True
 
     def pull(self):
         """The device's state back into the manager; waits for the current stream.  Captured steps are not replayed until the
         next push()."""
-        if not self._pushed:
+        if not self.has_state:
             raise _lib.WudaError(1, "the manager has the state already")
         cache = self.cache
         lengths, counts = self.lengths.tolist(), self.free_counts.tolist()
@@ -202,10 +202,10 @@ class CacheTables(StepTables):
                 req[name] = rows[slot, :-(-(lengths[slot] // RATIO) // epb)].tolist()
         for slot, req in cache.reqs.items():
             req["pos"] = lengths[slot] - 1
-        cache.on_device = self._pushed = False
+        cache.on_device = self.has_state = False
 
     def step(self, slots, new_tokens=None):
-        if not self._pushed:
+        if not self.has_state:
             raise _lib.WudaError(1, "the cache manager has the state: push() it first")
         return super().step(slots, new_tokens)
 
@@ -229,6 +229,6 @@ class _CacheReorder(BeamReorder):
         self._tables = tables
 
     def run(self, parents, slots, slots_out):
-        if not self._tables._pushed:
+        if not self._tables.has_state:
             raise _lib.WudaError(1, "the cache manager has the state: push() it first")
         return super().run(parents, slots, slots_out)
