@@ -202,3 +202,15 @@ def test_what_is_left_of_a_fork_is_forked_again(tokens):
     assert not m._owners["cmp"] and not m._owners["idx"]
     for name in ("swa", "cmp", "idx"):
         assert sorted(m._pools[name]._free) == list(range(30))
+
+
+def test_page_tables_are_not_answered_while_they_grow_on_the_device():
+    m = KVCacheManager(2, 4, 4, device="cpu")
+    a = m.alloc_request()
+    m.advance(a, 300)
+    pages = m.block_table("idx", [a])
+    m.on_device = True
+    with pytest.raises(RuntimeError):
+        m.block_table("idx", [a])
+    m.on_device = False
+    assert torch.equal(m.block_table("idx", [a]), pages)

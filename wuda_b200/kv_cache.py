@@ -87,7 +87,8 @@ class KVCacheManager:
         self.reqs = {}          # slot -> {"pos": last position, "swa"/"cmp"/"idx": page tables, "shared": tokens in shared pages,
                                 # "group": the slots that share them}
         self._owners = {"cmp": {}, "idx": {}}      # page -> requests that hold it, where they are more than one
-        self.on_device = False  # step tables on the device (step_tables.CacheTables) have the requests' state: nothing changes here
+        self.on_device = False  # step tables on the device (step_tables.CacheTables) have the requests' state: nothing changes here,
+                                # and the page tables here are old
 
     # ---- slot lifecycle: a new or reused slot starts with kv = 0, score = -inf
     def _reset_state(self, slot):
@@ -218,6 +219,7 @@ class KVCacheManager:
     main_state_rows = state_rows
 
     def block_table(self, name, slots):
+        self._need_state()
         bt = np.zeros((len(slots), self.max_pages), np.int32)
         for i, s in enumerate(slots):
             tab = self.reqs[s][name]
