@@ -9,6 +9,7 @@ import torch
 
 import wuda_b200._lib as L
 from wuda_b200.kv_cache import KVCacheManager
+from wuda_b200.step_tables import StepTables
 
 HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "wuda_b200.h")
 FAKE = 0x10000          # refused calls never read it
@@ -214,3 +215,10 @@ def test_page_tables_are_not_answered_while_they_grow_on_the_device():
         m.block_table("idx", [a])
     m.on_device = False
     assert torch.equal(m.block_table("idx", [a]), pages)
+
+
+@pytest.mark.parametrize("rows", [0, -1, 4097, 5000])
+def test_a_plan_of_more_rows_than_a_step_takes_is_refused(rows):
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    with pytest.raises(L.WudaError, match="max_rows"):
+        StepTables(i32(4), i32(4, 3), i32(4, 3), i32(4, 1), i32(2), i32(2), i32(2), max_rows=rows, max_tokens=8)

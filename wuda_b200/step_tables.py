@@ -20,6 +20,7 @@ from .ops import _int32, _on_current_device, _require, _stream
 
 _TOKEN_OUTPUTS = (("pos", torch.int64), ("q_pos", torch.int32), ("state_row", torch.int64), ("idx_dst", torch.int64),
                   ("cmp_dst", torch.int64), ("swa_dst", torch.int64))
+_MOST_ROWS = 4096       # of a step (wuda_step_tables)
 
 
 class StepTables:
@@ -41,7 +42,7 @@ class StepTables:
                             (cmp_entries_per_block, "cmp_entries_per_block"), (swa_entries_per_block, "swa_entries_per_block"),
                             (ratio, "ratio"), (ring_entries, "ring_entries"), (window, "window"), (topk, "topk")):
             _int32(value, name)
-        _require(max_rows >= 1 and max_tokens >= 0, "max_rows must be positive, max_tokens not negative")
+        _require(1 <= max_rows <= _MOST_ROWS and max_tokens >= 0, "max_rows must be in [1, %d], max_tokens not negative" % _MOST_ROWS)
         _require(_on_current_device(lengths), "the state must be on the current CUDA device")
         dev = lengths.device
 
