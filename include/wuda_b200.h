@@ -1102,6 +1102,7 @@ int wuda_step_tables(const wuda_step_tables_args* args, const int32_t* slots, co
  * beam's are not read).
  * Where a group has fewer than k continuations, the rest is (-inf, parent -1, token -1).
  *   finished_out[g, j] = the parent is finished, or the token is eos_token
+ * Outputs overlap neither inputs nor one another; with k = width, scores_out may be scores and finished_out finished.
  *
  * groups <= 256, width <= 32, k <= 64, vocab <= 2^24.  The result does not depend on how the work is split among CTAs of one
  * call of the same sizes, nor on the alignment of the rows: beams with the same logits get the same sums, bit for bit.

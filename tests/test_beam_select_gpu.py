@@ -5,12 +5,15 @@ and of its product with log2 e and that constant's (each 2^-24 of up to 104, whe
 exponential itself; a thread adds at most vocab / 256 + 32 terms one after the other.  So the sum, all of whose terms are positive, is off
 by at most (3 * 104 + 4 + vocab / 256 + 32) 2^-24 of itself, and its logarithm by as much.  The lists must be equal wherever the
 values are further apart than that on both sides; where beams or tokens tie exactly, always."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import wuda_b200 as wuda
 from step_oracle import beam_select
+from wuda_b200._lib import BeamSelectArgs, lib
 
 pytestmark = pytest.mark.gpu
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
@@ -293,3 +296,20 @@ def test_rows_of_one_value_and_sorted_rows_in_large_blocks(kind):
     scores = torch.full((7, 1), -0.75, device="cuda")
     for k in (5, 40):
         check(wuda.beam_select(logits, scores, k), logits, scores, k, exact=True)
+
+
+def test_scores_and_finished_in_place():
+    """Through the C ABI, with k = width: the beams' scores and flags are those after the selection."""
+    logits, scores = likely(5, 6, 20011, "bf16", seed=12)
+    finished = torch.zeros(5, 6, dtype=torch.bool, device="cuda")
+    finished[1, 2] = finished[4] = True
+    want = wuda.beam_select(logits, scores, finished=finished, eos_token=7)
+    parents, tokens = torch.empty(5, 6, dtype=torch.int32, device="cuda"), torch.empty(5, 6, dtype=torch.int32, device="cuda")
+    nbytes = lib.wuda_beam_select_workspace_bytes(5, 6, 20011, 6, 0)
+    workspace, counters = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    a = BeamSelectArgs(logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), finished.data_ptr(), scores.data_ptr(),
+                       parents.data_ptr(), tokens.data_ptr(), finished.data_ptr(), workspace.data_ptr(), nbytes, counters.data_ptr(),
+                       5, 6, 20011, 6, 7, 0)
+    assert lib.wuda_beam_select(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    for got, ref in zip((scores, parents, tokens, finished), want):
+        assert torch.equal(got, ref)

@@ -222,3 +222,12 @@ def test_a_plan_of_more_rows_than_a_step_takes_is_refused(rows):
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
     with pytest.raises(L.WudaError, match="max_rows"):
         StepTables(i32(4), i32(4, 3), i32(4, 3), i32(4, 1), i32(2), i32(2), i32(2), max_rows=rows, max_tokens=8)
+
+
+@pytest.mark.parametrize("change", [dict(scores_out=FAKE), dict(scores_out=FAKE + 124), dict(scores_out=FAKE - 60, k=4), dict(scores_out=FAKE - 252),
+                                    dict(finished=FAKE, finished_out=FAKE, eos_token=1), dict(finished=FAKE, finished_out=FAKE + 31, eos_token=1),
+                                    dict(finished=FAKE, finished_out=FAKE - 63, eos_token=1)])
+def test_beam_select_outputs_that_overlap_what_other_groups_still_read(change):
+    """scores float [8, 4] from FAKE to FAKE + 128, finished [8, 4] to FAKE + 32; outputs [8, k], k = 8 if not 4."""
+    a = select(**{**dict(groups=8, scores_out=2 * FAKE, finished_out=2 * FAKE), **change})
+    assert L.lib.wuda_beam_select(ctypes.byref(a), None) == INVALID and "overlap" in message(), message()

@@ -863,6 +863,14 @@ extern "C" int wuda_beam_select(const wuda_beam_select_args* args, void* stream)
     const int64_t need = wuda_beam_select_workspace_bytes(a.groups, a.width, a.vocab, a.k, a.logits_type);
     WUDA_REQUIRE(a.workspace_bytes >= need && aligned16(a.workspace), "the workspace needs %lld bytes on 16 bytes (got %lld)",
                  static_cast<long long>(need), static_cast<long long>(a.workspace_bytes));
+    // a group that ends writes its outputs while others still read their scores and flags
+    const int64_t beams = static_cast<int64_t>(a.groups) * a.width, best = static_cast<int64_t>(a.groups) * a.k;
+    const auto apart = [&](const void* out, const void* in, int64_t size) {
+        const auto o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in);
+        return (o == i && a.k == a.width) || o + best * size <= i || i + beams * size <= o;
+    };
+    WUDA_REQUIRE(apart(a.scores_out, a.scores, sizeof(float)), "scores_out must not overlap scores (but be them where k = width)");
+    WUDA_REQUIRE(!a.finished || apart(a.finished_out, a.finished, 1), "finished_out must not overlap finished (but be it where k = width)");
     DeviceInfo dev;
     if (const int st = current_device_info(&dev)) return st;
     Params p;
