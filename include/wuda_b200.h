@@ -64,7 +64,7 @@ typedef enum wuda_device_status {
     WUDA_DEV_BAD_SLOT = 161,        /* a request slot outside [-1, capacity), or in a batch for the second time: its row was left out */
     WUDA_DEV_NO_FREE_PAGE = 162,    /* a request found no free page: its row was left out */
     WUDA_DEV_BAD_LENGTH = 163,      /* a request's length does not fit its tables, the step's buffers or its group: its row was left out */
-    WUDA_DEV_BAD_PARENT = 164       /* a beam's parent is no live beam of its group: the beam was given none */
+    WUDA_DEV_BAD_PARENT = 164       /* a beam's parent is outside [-1, width): the beam was given none */
 } wuda_device_status;
 
 /* Library version (major*10000 + minor*100 + patch). */
@@ -1047,6 +1047,9 @@ int wuda_indexer_topk_host_pages(wuda_indexer_plan* plan, const void* q_host, co
  *   token i      of the row stands at position pos = old + i.  idx_dst / cmp_dst: entry (pos + 1) / ratio - 1 through the page table
  *                where (pos + 1) % ratio == 0; swa_dst: ring entry pos % window; state_row: slot * ring_entries + pos % ring_entries.
  *                -1 where there is nothing to write, and where a later token of the row takes the same ring entry.
+ *                More than one token to a row is for a caller's own prefill: all tokens get the destinations of their compressed
+ *                entries, the last ones only a ring row.  The cache writers of this library take one token per request and read
+ *                the tokens in front of it from the ring; a token without a ring row they skip, its compressed entry included.
  *   row values   n_compressed = entries(now), cmp_lengths = min(n_compressed, topk), swa_lengths = min(now, window), the window's pool
  *                entries in the order of their positions (-1 behind them), block tables with zeros behind the pages held
  *   token_starts the first token of each row, then their number; token values behind the last token are left as they were

@@ -8,9 +8,9 @@
 // each: rows of the states, entries of one page of a pool); a scan over the forks numbers the pieces and the CTAs take them in turn.
 //
 // What bounds it: about 5 us of launch, slots, lengths, page tables and first loads, then HBM.  Per launch in a graph: 4 beams with two
-// forks (0.8 MB moved) 5.7 us; 16 x 8 beams, 64 forks (32 MB) 9.9; 8 x 32 beams, 160 MB 31.0 - 5.2 TB/s with the start, 6.2 without,
+// forks (0.8 MB moved) 5.7 us; 16 x 8 beams, 64 forks (32 MB) 9.9; 8 x 32 beams, 160 MB 31.3 - 5.1 TB/s with the start, 6.1 without,
 // where a copy reaches 6.54.  Four loads of 16 bytes per thread and five CTAs of 256 threads per SM: four CTAs, or eight loads, were
-// 1-3 us slower at 160 MB; streaming stores 31.3 us, plain ones 34.6 (they push out of L2 what is still to be read).
+// 1-3 us slower at 160 MB; plain stores took 34.6 us (they push out of L2 what is still to be read).
 #include "batch_slots.cuh"
 
 namespace wuda {

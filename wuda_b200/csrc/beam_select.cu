@@ -23,11 +23,11 @@
 // The CTA that completes a group's counter merges its lists the same way: the k-th largest of the maxima over 64 or 128 shares of the
 // lists' first candidates bounds what can be among the k best, and the few that pass are ranked by counting.
 //
-// What bounds it (per launch in a graph, against a copy's 6.54 TB/s): small calls the chain of launch, a chunk's loads, its fence and
-// counter, and the merge's three round trips to L2 - 4 rows x 32000 bf16 8.2 us, of which the merge is 4.  Large ones the stream and what
-// goes on beside it: 512 rows x 131072 bf16 (134 MB) 32.6-33.7 us, 20.5 at the copy's rate.  Loads in this pattern alone take 22 us, the
-// exponentials 2 on top, raising the bounds and notes 2 each, the merge 4.  256 rows x 131072 fp32, half the elements for the same
-// bytes: 31.2.  Rows off 16 bytes: 38.9.
+// What bounds it (per launch in a graph, against a copy's 6.54 TB/s; plain calls one after the other take 0.4 to 1.3 us more): small calls
+// the chain of launch, a chunk's loads, its fence and counter, and the merge's three round trips to L2 - 4 rows x 32000 bf16 8.2 us, of
+// which the merge is 4.  Large ones the stream and what goes on beside it: 512 rows x 131072 bf16 (134 MB) 32.3 us with k = 8 and 34.3 with
+// 16, 20.5 at the copy's rate.  Loads in this pattern alone take 22 us, the exponentials 2 on top, raising the bounds and notes 2 each,
+// the merge 4.  256 rows x 131072 fp32, half the elements for the same bytes: 30.6.  The bf16 rows off 16 bytes: 39.2.
 // More warps were worth more than anything else: a ring of bulk copies in shared memory left room for 5 or 6 CTAs per SM instead of 7
 // (49-54 us instead of 40 at the time), and exponentials by polynomials for a part of the elements took more slots than they freed (42-47).
 // Asking L2 for the tiles after the next one made it slower (35.4 to 38.5 us for two to eight tiles ahead, against 35.0 at the time).
@@ -798,13 +798,16 @@ __global__ void __launch_bounds__(kThreads, 896 / kThreads) beam_select_kernel(c
 
 // How the rows are cut, into chunks of whole tiles and lists that the merge can hold.
 //   Up to 148 rows of more work than a tile of 128 threads per SM: CTAs of 512 threads, one per SM at most.  Fewer and longer lists make
-//   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 11.7 us (13.0 in CTAs of 128), 128 rows x
-//   131072 bf16, k = 16: 15.6 (17.4); 64 rows x 131072 fp32, k = 4: 13.0 (14.0).
+//   the merge shorter, and a CTA alone on its SM needs the threads.  7 x 5 rows x 100003 fp16: 11.7 us (13.1 in CTAs of 128), 128 rows x
+//   131072 bf16, k = 16: 16.0 (17.8); 64 rows x 131072 fp32, k = 4: 13.1 (14.2).  On the other side of both limits 152 rows x 131072
+//   bf16: 17.9 us in CTAs of 128, 24.4 in those of 512; 4 rows of them 9.2 (8.8).
 //   So, too, where the lists leave fewer than two fifths of the places of CTAs of 128 threads (wide groups, large k): 8 x 32 rows x
-//   131072 bf16, k = 64: 41.7 us (47.9 in CTAs of 128), 6 x 32 rows, k = 32: 28.2 (35.0); at half of them, 16 x 32 rows, k = 64, 76.3 (58.4).
-//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 32.6 us in two chunks a row,
-//   35.0 in three, 48.2 with 512 threads; 4 rows x 32000 bf16: 8.2 us in eight chunks of a tile (9.0 with 512 threads).  Rows that
-//   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 50.9 -> 39.7 us.
+//   131072 bf16, k = 64: 41.7 us (49.0 in CTAs of 128), 12 x 32: 59.1 (70.1), 6 x 32 rows, k = 32: 28.3 (35.0).  Beyond that, 16 x 32 rows,
+//   k = 64: 60.0 us in CTAs of 128, 76.2 in those of 512 (13 x 32, next to the limit, would gain: 78.0, 60.0).
+//   Otherwise CTAs of 128 threads, as many as are resident together (seven per SM).  512 rows x 131072 bf16: 32.3 us in two chunks a row,
+//   35.1 in three, 48.4 with 512 threads; 4 rows x 32000 bf16: 8.0 us in eight chunks of a tile (8.7 with 512 threads).  Rows that
+//   fill half of the places or little more leave the others empty, so they are cut in three: 600 rows x 131072 51.1 -> 39.8 us, 800 rows
+//   52.4 -> 49.3; 960 rows in one chunk 53.9 (56.1 in three).
 struct Cut {
     int threads, chunks, chunk_vectors;
 };

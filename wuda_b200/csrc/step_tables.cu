@@ -11,8 +11,9 @@
 // all have to be waited for once.
 //
 // What bounds it is that chain: launch, slots, lengths, scan, tables or free pages, stores - four dependent round trips to L2.  Per launch
-// in a graph: 1 request 4.2 us, 64 requests of 32768 tokens 4.2, 128 of a million tokens (tables of 4096 pages, 6.5 MB read and
-// written: 1.0 us at 6.54 TB/s) 5.7, 37 requests with 65521 tokens between them 6.1.  In one CTA the latter two took 447 and 150 us.
+// in a graph, state in place / to other tensors: 1 request 4.0 / 4.1 us, 64 requests of 32768 tokens 4.6 / 4.2, 128 of a million tokens
+// (tables of 4096 pages, 6.5 MB read and written: 1.0 us at 6.54 TB/s) 6.2 / 5.5, 37 requests with 65521 tokens between them - / 6.1 (in
+// place costs a counter, a barrier and a write behind both).  In one CTA the latter two took 447 and 150 us.
 // kPiece = 256: eight loads of a lane in flight, and 128 x 2 x 16 pieces give each of the 2368 warps two.
 #include "batch_slots.cuh"
 

@@ -127,7 +127,9 @@ class StepTables:
           swa_indices int32 [rows, window]; idx_block_table, cmp_block_table int32 [rows, pages]
         What lies behind the last token and the last row is left as it was.  A row that cannot be served (a slot given twice,
         no free page, a context beyond the tables) is reported in status_word and left out: positions 0, destinations -1,
-        lengths 0; its state stays."""
+        lengths 0; its state stays.
+        More than one token to a request is for a caller's own prefill: only a request's last tokens get a ring row, and the cache
+        writers of this package skip those without one."""
         if _ops._fast.step_tables(self._address, slots, new_tokens, self.max_rows, self._device, self._status):
             return self.out
         rows = slots.numel()
